@@ -368,6 +368,45 @@ int rdkv_argmax_advance_word(const void *logits, int n, int dtype, int64_t *toke
 int rdkv_gemv(const void *W, int64_t w_stride_row, const void *x, int x_dtype, const void *bias, int N,
               int K, int dtype, void *y, void *stream);
 
+/* ---- 4-bit weights with group scales ----------------------------------------------------
+ * No counterpart in the reference, which projects with the model's own weights; the products stand
+ * beside rdkv_gemv* and read a quarter of their bytes.  A matrix W [N, K] is held as
+ *   W[n, k] = (q[n, k] - zero[n, g]) * scale[n, g],  q and zero in 0 .. 15, g = k / group,
+ * group 32, 64 or 128 (the last of a row may be short), in a layout of the library's own:
+ * `codes` (16-byte aligned, rdkv_w4_codes_bytes) and `scales` (rdkv_w4_scale_words words: fp32 with the
+ * zero point in the four lowest mantissa bits, so scales keep 20 significant bits).  `dtype`, fp16 or
+ * bf16, is the activations'; the same codes and scales serve both. */
+int64_t rdkv_w4_codes_bytes(int N, int K);
+int64_t rdkv_w4_scale_words(int N, int K, int group);
+/* Round to nearest by groups: lo = min(0, group), hi = max(0, group), scale = (hi - lo) / 15 (kept to 20 bits;
+ * below 2^-120: a group of zeros), zero = rint(-lo / scale), q = clamp(rint(W / scale) + zero), all in fp32.
+ * A group that holds a NaN or an infinity has scale NaN: every product with it is NaN. */
+int rdkv_w4_quantize(const void *W, int64_t w_stride_row, int N, int K, int group, int dtype, void *codes,
+                     uint32_t *scales, void *stream);
+/* A matrix quantized elsewhere: q u8 [N, K] (the low four bits count), scale [N, groups] of scale_dtype, zero u8
+ * [N, groups] or NULL (then 8, the middle of the codes). */
+int rdkv_w4_pack(const uint8_t *q, int64_t q_stride_row, const void *scale, int scale_dtype,
+                 int64_t scale_stride_row, const uint8_t *zero, int64_t zero_stride_row, int N, int K, int group,
+                 void *codes, uint32_t *scales, void *stream);
+/* The values, rounded to `dtype`: out [N, K]. */
+int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, int K, int group, int dtype, void *out,
+                    int64_t out_stride_row, void *stream);
+/* y[m, n] = sum_k x[m, k] * W[n, k] (+ bias[n]): x [M, K] of x_dtype = `dtype`, or fp32 (rounded to `dtype` first), y [M, N]
+ * and bias [N] of `dtype`; fp32 accumulation in a fixed order.  Any M, N, K.  The workspace (at most
+ * rdkv_w4_linear_workspace_bytes, 16-byte aligned) is used for rows that are fp32, misaligned or no multiple of 8
+ * long, unless M is 1 and K at most 32768; it may be NULL otherwise. */
+int64_t rdkv_w4_linear_workspace_bytes(int M, int K);
+int rdkv_w4_linear(const void *codes, const uint32_t *scales, const void *x, int x_dtype, int64_t x_stride_row,
+                   const void *bias, int M, int N, int K, int group, int dtype, void *y, int64_t y_stride_row,
+                   void *workspace, int64_t workspace_bytes, void *stream);
+/* rdkv_gemv_norm and rdkv_gemv_silu over 4-bit weights: one row, the operation in front of the product folded into
+ * the staging of the row, with the same roundings.  K at most 32768. */
+int rdkv_w4_linear_norm(const void *codes, const uint32_t *scales, const void *x, const void *delta,
+                        const void *norm_weight, float eps, void *residual_out, const void *bias, int N, int K,
+                        int group, int dtype, void *y, void *stream);
+int rdkv_w4_linear_silu(const void *codes, const uint32_t *scales, const void *gate, const void *up,
+                        const void *bias, int N, int K, int group, int dtype, void *y, void *stream);
+
 /* ---- triton_rope.py : fused_rope (:86-108) -------------------------------- */
 /* Half-split rotary embedding of one decode step, in place: for every head of q [H_q, D] and
  * k [H_kv, D] (dtype code `dtype`, head strides in elements) and i < D/2:

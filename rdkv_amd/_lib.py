@@ -108,6 +108,15 @@ SIGNATURES = {
     "rdkv_gemv": (I, [P, L, P, I, P, I, I, I, P, P]),
     "rdkv_gemv_norm": (I, [P, L, P, P, P, F, P, P, I, I, I, P, P]),
     "rdkv_gemv_silu": (I, [P, L, P, P, P, I, I, I, P, P]),
+    "rdkv_w4_codes_bytes": (L, [I, I]),
+    "rdkv_w4_scale_words": (L, [I, I, I]),
+    "rdkv_w4_quantize": (I, [P, L, I, I, I, I, P, P, P]),
+    "rdkv_w4_pack": (I, [P, L, P, I, L, P, L, I, I, I, P, P, P]),
+    "rdkv_w4_dequant": (I, [P, P, I, I, I, I, P, L, P]),
+    "rdkv_w4_linear_workspace_bytes": (L, [I, I]),
+    "rdkv_w4_linear": (I, [P, P, P, I, L, P, I, I, I, I, I, P, L, P, L, P]),
+    "rdkv_w4_linear_norm": (I, [P, P, P, P, P, F, P, P, I, I, I, I, P, P]),
+    "rdkv_w4_linear_silu": (I, [P, P, P, P, P, I, I, I, I, P, P]),
     "rdkv_decode_fused_merge": (I, [P, I, I, I, P, L, P, P, L, P]),
     "rdkv_pack_layer_plan_ints": (L, [I, L]),
     "rdkv_pack_layer_plan": (I, [P, I, L, P, I, L, I, L, I, P, L, P, L, P, P]),
