@@ -407,6 +407,39 @@ int rdkv_w4_linear_norm(const void *codes, const uint32_t *scales, const void *x
 int rdkv_w4_linear_silu(const void *codes, const uint32_t *scales, const void *gate, const void *up,
                         const void *bias, int N, int K, int group, int dtype, void *y, void *stream);
 
+/* ---- sampling of the next token ---------------------------------------------------------
+ * No counterpart in the reference, which decodes greedily (rdkv_argmax_advance).  Per row of logits l, with
+ * w_i = exp((l_i - max) / temperature) and the tokens in descending order (equal logits by index):
+ *   top_k > 0: the first top_k tokens stay; top_p < 1: of those, the shortest run from the front whose sum is at least
+ *   top_p of theirs; min_p > 0: tokens with w_i >= min_p; the first token always stays;
+ *   token = the first one whose running sum exceeds uniform * the sum of those that stay (uniform in [0, 1)),
+ *   logprob = the log of its share of that sum.
+ * A temperature that is not above 0 takes the largest logit (logprob 0).  NaN and -inf are masked; a logit of +inf
+ * leaves the others without weight; a row with nothing left has token -1 and logprob -inf.  Weights and sums are
+ * held in 64 bits: the same token whatever the batch.  A member of RdkvSampling that is not NULL holds one value per
+ * row (device memory), else its _value counts. */
+typedef struct RdkvSampling {
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+  float temperature_value;
+  int32_t top_k_value;
+  float top_p_value;
+  float min_p_value;
+} RdkvSampling;
+int64_t rdkv_sample_workspace_bytes(int rows);
+/* logits [rows, vocab] of `dtype` (any row stride, vocab at most 2^24), uniform [rows], token [rows], logprob [rows] or NULL. */
+int rdkv_sample_rows(const void *logits, int64_t stride_row, int rows, int vocab, int dtype, const float *uniform,
+                     const RdkvSampling *sampling, int64_t *token, float *logprob, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+/* rdkv_argmax_advance[_word] with a sampled token: one row; the uniform is uniform[uniform_index[0]] (device int64, read
+ * before the counters advance; held to 0 .. n_uniform - 1), so a captured step takes the next one on each replay. */
+int rdkv_sample_advance(const void *logits, int vocab, int dtype, const float *uniform, int n_uniform,
+                        const int64_t *uniform_index, const RdkvSampling *sampling, int64_t *token,
+                        int64_t *counter_a, int64_t *counter_b, int32_t *counts, int n_counts, uint64_t *word,
+                        uint32_t tag_base, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- triton_rope.py : fused_rope (:86-108) -------------------------------- */
 /* Half-split rotary embedding of one decode step, in place: for every head of q [H_q, D] and
  * k [H_kv, D] (dtype code `dtype`, head strides in elements) and i < D/2:

@@ -21,6 +21,14 @@ class RdkvTailScores(ctypes.Structure):
                 ("next_stride_h", c_int64), ("q_block_start", ctypes.c_int32), ("block", ctypes.c_int32),
                 ("q_rotated_stride_tok", c_int64)]
 
+
+class RdkvSampling(ctypes.Structure):
+    """``RdkvSampling`` of include/rdkv.h (read by the library during the call)."""
+    _fields_ = [("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p),
+                ("temperature_value", c_float), ("top_k_value", ctypes.c_int32), ("top_p_value", c_float),
+                ("min_p_value", c_float)]
+
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "librdkv_hip.so")
 NATIVE_PATH = os.path.join(_PKG, "_native.so")
@@ -117,6 +125,9 @@ SIGNATURES = {
     "rdkv_w4_linear": (I, [P, P, P, I, L, P, I, I, I, I, I, P, L, P, L, P]),
     "rdkv_w4_linear_norm": (I, [P, P, P, P, P, F, P, P, I, I, I, I, P, P]),
     "rdkv_w4_linear_silu": (I, [P, P, P, P, P, I, I, I, I, P, P]),
+    "rdkv_sample_workspace_bytes": (L, [I]),
+    "rdkv_sample_rows": (I, [P, L, I, I, I, P, P, P, P, P, L, P]),
+    "rdkv_sample_advance": (I, [P, I, I, P, I, P, P, P, P, P, P, I, P, ctypes.c_uint32, P, L, P]),
     "rdkv_decode_fused_merge": (I, [P, I, I, I, P, L, P, P, L, P]),
     "rdkv_pack_layer_plan_ints": (L, [I, L]),
     "rdkv_pack_layer_plan": (I, [P, I, L, P, I, L, I, L, I, P, L, P, L, P, P]),
