@@ -597,11 +597,12 @@ def _compress_block(*, target_kv: List[Tensor], query_block: List[Tensor], token
 
 def greedy_decode_blockwise(*, model, dual_cache: TriZoneCache, next_token_logits: Tensor, max_new_tokens: int,
                             eos_token_ids, primary_device: torch.device, decode_position_start: int,
-                            config: BlockwiseRDKVConfig, use_cuda_graph: bool = False
+                            config: BlockwiseRDKVConfig, use_cuda_graph: bool = False, weights=None
                             ) -> Tuple[List[int], Dict[str, Any]]:
     """Greedy decode that keeps the generated tokens as immutable packed blocks
     (blockwise_decode.py:1124-2260): same keyword arguments, return value (token ids and the report
-    with the reference's keys) and compression schedule.
+    with the reference's keys) and compression schedule.  ``weights``: what the steps project with, in place of
+    the model's own (``fast_decode.quantize_weights``).
 
     The raw tail holds at most two blocks.  Every step attends over [prompt cache | compressed
     blocks | raw tail] in two launches per layer (the compressed blocks are further sources of the
@@ -630,7 +631,7 @@ def greedy_decode_blockwise(*, model, dual_cache: TriZoneCache, next_token_logit
     if dev.type != "cuda":
         raise RuntimeError("blockwise packed decode requires CUDA")
     eos_set = {int(t) for t in eos_token_ids if t is not None}
-    W = pre_extract_weights(model)
+    W = pre_extract_weights(model) if weights is None else weights
     model_dtype = next(model.parameters()).dtype
     h_q, h_kv, groups, D, L = W.num_heads, W.num_kv_heads, W.num_kv_groups, W.head_dim, W.num_layers
     block = int(config.block_size)

@@ -14,6 +14,7 @@ fused streaming kernel, and with ``use_cuda_graph`` the whole step is one HIP gr
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Tuple
@@ -21,11 +22,13 @@ from typing import List, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from . import _lib, k_kernel
+from . import _lib, k_kernel, weight_quant
 from .k_kernel import INV_SQRT_D, k_mixed_qk_dot_into
 from .packing import PackedKVLayer
+from .sampling import Sampling, _sample_advance, sample_tokens
 from .stream_cache import StreamCache, build_stream_cache, decode_attn_fused
 from .v_kernel import _weighted_sum_with_new_zone, v_dequant_weighted_sum_dispatch_into  # noqa: F401
+from .weight_quant import QuantizedWeight
 
 
 def _rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: Optional[torch.Tensor] = None,
@@ -98,12 +101,14 @@ def _argmax_advance(logits: torch.Tensor, token: torch.Tensor, position: Optiona
         word.tag_base if word is not None else 0, _lib.stream_of(dev)))
 
 
-def _linear_row(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+def _linear_row(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``F.linear(x.to(weight.dtype), weight, bias)`` for the single activation row of a decode
     step (fast_decode.py:1650-1656, 1785-1786, 1797-1804, 1826): one pass over the weights with
     ``rdkv_gemv`` when the shape allows it (fp16 / bf16 weights, K a multiple of 512 up to 32768,
     16-byte aligned rows; x of the weights' type or fp32, which the kernel rounds while staging
-    it), the library GEMM otherwise."""
+    it), the library GEMM otherwise.  A ``QuantizedWeight`` goes to its own product."""
+    if isinstance(weight, QuantizedWeight):
+        return weight_quant.linear(x, weight, bias)
     dev = _lib.require_device(x, weight)          # no CPU path: the library product below is the GPU's too
     N, K = weight.shape
     ok = (x.numel() == K and x.dtype in (weight.dtype, torch.float32)
@@ -132,11 +137,15 @@ def _gemv_weight_ok(weight: torch.Tensor, bias: Optional[torch.Tensor], k_max: i
 
 
 def _norm_linear_row(h: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float,
-                     weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                     weight, bias: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Residual add, RMSNorm and projection of one activation row (fast_decode.py:1640-1656 and
     1786-1798): returns ``(F.linear(rms_norm(h + delta), weight, bias), h + delta)``.  One launch
-    (``rdkv_gemv_norm``: the norm is folded into the staging of the row) when the shapes allow it,
-    ``_rms_norm`` + ``_linear_row`` otherwise."""
+    (``rdkv_gemv_norm`` or ``rdkv_w4_linear_norm``: the norm is folded into the staging of the row) when the
+    shapes allow it, ``_rms_norm`` + ``_linear_row`` otherwise."""
+    if isinstance(weight, QuantizedWeight) and weight.K <= 32768 and norm_weight.dtype == weight.dtype:
+        return weight_quant.norm_linear(h, delta, norm_weight, eps, weight, bias)
+    if isinstance(weight, QuantizedWeight):
+        return weight_quant.linear(_rms_norm(h, norm_weight, eps, delta=delta, residual_out=h), weight, bias), h
     dev = _lib.require_device(h, weight)
     N, K = weight.shape
     fused = (_gemv_weight_ok(weight, bias, 8192) and h.numel() == K and h.dtype == weight.dtype
@@ -154,9 +163,13 @@ def _norm_linear_row(h: torch.Tensor, delta: Optional[torch.Tensor], norm_weight
     return y, h_new
 
 
-def _silu_linear_row(gate: torch.Tensor, up: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+def _silu_linear_row(gate: torch.Tensor, up: torch.Tensor, weight) -> torch.Tensor:
     """``F.linear(F.silu(gate) * up, weight)`` for one row (fast_decode.py:1803-1804): one launch
-    (``rdkv_gemv_silu``) when the shapes allow it, ``_silu_mul`` + ``_linear_row`` otherwise."""
+    (``rdkv_gemv_silu`` or ``rdkv_w4_linear_silu``) when the shapes allow it, ``_silu_mul`` + ``_linear_row``
+    otherwise."""
+    if isinstance(weight, QuantizedWeight):
+        return (weight_quant.silu_linear(gate, up, weight) if weight.K <= 32768
+                else weight_quant.linear(_silu_mul(gate, up), weight))
     dev = _lib.require_device(gate, up, weight)
     N, K = weight.shape
     fused = (_gemv_weight_ok(weight, None, 32768) and gate.numel() == K and up.numel() == K
@@ -437,8 +450,25 @@ def pre_extract_weights(model) -> PreExtractedWeights:
     return weights
 
 
+def quantize_weights(model, group_size: int = 128, lm_head: bool = True) -> PreExtractedWeights:
+    """The model's weights for the decode loop with every projection (and, unless ``lm_head`` is False, the
+    LM head) as 4-bit codes with one scale and zero point per ``group_size`` columns
+    (``weight_quant.quantize_weight``), for ``greedy_decode_fast(..., weights=...)``.  The concatenated
+    q / k / v and gate / up matrices are quantized as they are; norms, embedding and biases stay.  fp16 or bf16 models;
+    the model keeps its own weights."""
+    W = pre_extract_weights(model)
+    _lib.require_device(W.lm_head_weight)
+    layers = [dataclasses.replace(lw, qkv_weight=weight_quant.quantize_weight(lw.qkv_weight, group_size),
+                                  o_proj_weight=weight_quant.quantize_weight(lw.o_proj_weight, group_size),
+                                  gate_up_weight=weight_quant.quantize_weight(lw.gate_up_weight, group_size),
+                                  down_proj_weight=weight_quant.quantize_weight(lw.down_proj_weight, group_size))
+              for lw in W.layers]
+    head = weight_quant.quantize_weight(W.lm_head_weight, group_size) if lm_head else W.lm_head_weight
+    return dataclasses.replace(W, layers=layers, lm_head_weight=head)
+
+
 class _DecodeStep:
-    """One greedy decode step over device-resident state, written so that the same calls run
+    """One decode step over device-resident state, written so that the same calls run
     eagerly or are captured once into a HIP graph: the token, its position, the zone C write row
     and the zone C token counts live in device tensors that the step itself advances, so a replay
     needs no argument from the host.  Per layer, six launches: q/k/v GEMV with the residual add
@@ -460,6 +490,8 @@ class _DecodeStep:
         self.hidden = None      # final-normalized hidden state [1,1,hidden] of the last step
         self.logits = None      # [1,1,vocab] of the last step
         self.word = None        # takes the chosen token to the host
+        self.sampling = None    # how the token is drawn (None: the largest logit), and the numbers it is drawn with,
+        self.uniforms = None    # one per row of zone C
         self.rope = None        # cos / sin halves of the next step, where they were formed ahead
         self.stream_row = None  # a residual stream row, for the rotary embedding's dtype and device
 
@@ -496,7 +528,11 @@ class _DecodeStep:
             delta = _silu_linear_row(gate, up, lw.down_proj_weight)
         self.hidden = _rms_norm(h, W.final_norm_weight, W.final_norm_eps, delta=delta, residual_out=h)
         self.logits = _linear_row(self.hidden, W.lm_head_weight)
-        _argmax_advance(self.logits, self.token, self.position, self.write_row, self.n_new, self.word)
+        if self.sampling is None:
+            _argmax_advance(self.logits, self.token, self.position, self.write_row, self.n_new, self.word)
+        else:
+            _sample_advance(self.logits, self.token, self.sampling, self.uniforms, self.position, self.write_row,
+                            self.n_new, self.word)
 
     def rope_ahead(self) -> None:
         """cos / sin of ``position``.  They do not depend on the token: formed behind the step before, the model's
@@ -531,7 +567,8 @@ def _layer_stream_caches(dual_cache, num_kv_groups: int) -> List[StreamCache]:
 
 def greedy_decode_fast(model, dual_cache, next_token_logits, max_new_tokens, eos_token_ids, primary_device,
                        decode_position_start, use_cuda_graph=False, return_logits=False,
-                       next_token_hidden=None, logits_observer=None, hidden_observer=None):
+                       next_token_hidden=None, logits_observer=None, hidden_observer=None, weights=None,
+                       sampling: Optional[Sampling] = None, uniforms: Optional[torch.Tensor] = None):
     """Greedy decode over a packed prompt cache without ``model.forward`` (fast_decode.py:731-1860):
     same arguments, return value, observer protocol and errors.
 
@@ -545,15 +582,26 @@ def greedy_decode_fast(model, dual_cache, next_token_logits, max_new_tokens, eos
     ``use_cuda_graph``: step 0 runs eagerly, then the whole step - every layer, LM head and argmax
     - is captured as ONE HIP graph and replayed; token, position and zone C length are device
     state that the graph advances, so no per-length or per-layer graphs are needed.  As in the
-    reference, observers and ``return_logits`` need the eager path."""
+    reference, observers and ``return_logits`` need the eager path.
+
+    ``weights``: what the steps project with, in place of the model's own (``quantize_weights``).
+    ``sampling`` (``sampling.Sampling``) with ``uniforms`` (fp32 in [0, 1) on the model's device, at least
+    ``max_new_tokens`` of them, token i is drawn with the i-th): tokens are sampled instead of taking the argmax,
+    the first one from ``next_token_logits`` too.  Logits that leave no token to draw raise ``RuntimeError``."""
     eos_set = {int(t) for t in eos_token_ids if t is not None}
     if (return_logits or logits_observer is not None or hidden_observer is not None) and use_cuda_graph:
         raise NotImplementedError("logit observation is only supported under eager decode (use_cuda_graph=False)")
     if hidden_observer is not None and next_token_hidden is None:
         raise ValueError("hidden_observer requires next_token_hidden")
-    W = pre_extract_weights(model)
+    if (sampling is None) != (uniforms is None):
+        raise ValueError("sampling needs its uniforms, and uniforms their sampling")
+    W = pre_extract_weights(model) if weights is None else weights
     dev = torch.device(primary_device)
-    _lib.require_device(W.lm_head_weight)
+    _lib.require_device(W.lm_head_weight.codes if isinstance(W.lm_head_weight, QuantizedWeight) else W.lm_head_weight)
+    if uniforms is not None:
+        assert uniforms.dim() == 1 and uniforms.dtype == torch.float32 and uniforms.numel() >= max_new_tokens, \
+            f"uniforms: at least {max_new_tokens} fp32 numbers, got {tuple(uniforms.shape)} {uniforms.dtype}"
+        assert uniforms.device == W.device, f"uniforms: on {uniforms.device}, the model on {W.device}"
     assert W.head_dim == 128, f"the packed format is defined for head_dim 128, got {W.head_dim}"
     assert len(dual_cache.packed) == W.num_layers, "one packed layer per decoder layer"
     model_dtype = next(model.parameters()).dtype
@@ -577,12 +625,23 @@ def greedy_decode_fast(model, dual_cache, next_token_logits, max_new_tokens, eos
     graph = None
     with torch.inference_mode():
         position = int(decode_position_start)
-        step_state.reset(next_token_logits.argmax(dim=-1, keepdim=True).to(dev), position)
+        if sampling is None or max_new_tokens < 1:
+            first = next_token_logits.argmax(dim=-1, keepdim=True)
+        else:
+            first, _ = sample_tokens(next_token_logits.to(W.device), uniforms[:1], temperature=sampling.temperature,
+                                     top_k=sampling.top_k, top_p=sampling.top_p, min_p=sampling.min_p)
+            # (the number behind the last token's is asked for by the last step, whose choice nobody reads)
+            step_state.sampling, step_state.uniforms = sampling, uniforms[1:max_new_tokens].contiguous()
+            if max_new_tokens == 1:
+                step_state.uniforms = uniforms[:1].contiguous()
+        step_state.reset(first.to(dev), position)
         step_state.word = _lib.step_word(step_state.token.device, max_new_tokens, position)
         for step in range(max_new_tokens):
             token_id = step_state.word.read(position + step) if step else None
             if token_id is None:
                 token_id = int(step_state.token.item())
+            if token_id < 0:
+                raise RuntimeError(f"step {step}: the logits leave no token to draw")
             if logits_observer is not None:
                 logits_observer(step, next_token_logits if step == 0 else step_state.logits[:, -1, :], token_id,
                                 token_id in eos_set)
