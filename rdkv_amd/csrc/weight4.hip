@@ -242,6 +242,13 @@ struct RowSource {
   int aligned;                 // a, b, c and residual_out are 16-byte aligned
 };
 
+// g / (1 + exp(-g)) with the hardware's exponential and reciprocal (an ulp each, 2^-17 in all at the steepest: a 64th of
+// the rounding to 16 bits that follows).  Every workgroup stages the whole row: with the library's exponential and the
+// correctly rounded division the staging of 14336 columns took 4 of 12 us.
+__device__ __forceinline__ float silu(float g) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
+}
+
 // Eight elements of a 16-bit row from element k on; what lies behind the row is zero.
 template <int dtype>
 __device__ __forceinline__ void row8(const void *row, int k, int K, int aligned, float (&f)[8]) {
@@ -264,21 +271,49 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
 }
 
 // One activation row.  A workgroup takes row tiles in turn and its wavefronts share a tile's columns (runs of
-// column tiles); the wavefronts' sums meet in LDS and are added in their order.
-template <int dtype, int MODE, int GPC, int WAVES>
+// column tiles); the wavefronts' sums are kept in LDS and added in their order, kKept tiles at a time, so that between
+// them no wavefront waits for another.
+constexpr int kKept = 16;
+template <int dtype, int MODE, int GPC, int WAVES, int U>
 __global__ void __launch_bounds__(64 * WAVES)
 w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, RowSource src,
               const uint16_t *__restrict__ bias, int N, int K, int n_tiles_n, int n_tiles_k, uint16_t *__restrict__ y) {
   extern __shared__ u32x4 lds[];       // the row (16 pieces of 8 per column tile), then a sum per group
-  __shared__ float s_red[2][WAVES][16];
+  __shared__ float s_red[kKept][WAVES][16];
   __shared__ float s_part[WAVES];
   u32x4 *xs = lds;
   float *sums = reinterpret_cast<float *>(lds + n_tiles_k * 16);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane >> 4, n = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, n = lane & 15;
   const int pieces = n_tiles_k * 16;
   constexpr int PPG = 16 / GPC;        // pieces per group
+  // A wavefront walks its run of every row tile in steps of U column tiles; the loads of the next step are issued
+  // before the current one is consumed, those of the first before the row is staged.
+  struct Cur { int tn, step; };
+  struct Piece { u32x4 q[U]; uint32_t w[U][GPC]; };
+  // (every wavefront makes the same number of steps a tile: the barriers are met by all together)
+  const int run = (n_tiles_k + WAVES - 1) / WAVES, steps = (run + U - 1) / U;
+  const int k_begin = min(wave * run, n_tiles_k), k_end = min(k_begin + run, n_tiles_k);
+  auto next = [&](Cur c) __attribute__((always_inline)) -> Cur {
+    if (c.step + 1 < steps) return Cur{c.tn, c.step + 1};
+    return Cur{c.tn + (int)gridDim.x, 0};
+  };
+  auto load = [&](Cur c, Piece &p) __attribute__((always_inline)) {
+    const int64_t tile = (int64_t)c.tn * n_tiles_k;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = tile + min(k_begin + c.step * U + u, n_tiles_k - 1);     // (behind the run: loaded, not used)
+      p.q[u] = load_stream(codes + at * 64 + lane);
+#pragma unroll
+      for (int g = 0; g < GPC; ++g) p.w[u][g] = scales[(at * GPC + g) * 16 + n];
+    }
+  };
+  Piece pa, pb;
+  Cur ca{(int)blockIdx.x, 0};
+  if (ca.tn < n_tiles_n) load(ca, pa);
   float rs = 0.0f;
+  float norm0[8];                      // the norm weight of the thread's first piece, asked for ahead of the barrier
   if (MODE == kNorm) {
+    row8<dtype>(src.c, min(8 * tid, K - 1), K, src.aligned, norm0);
     float ss = 0.0f;
     for (int i = tid; i < pieces; i += 64 * WAVES) {
       float f[8];
@@ -317,7 +352,12 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
       for (int j = 0; j < 8; ++j) f[j] = 8 * i + j < K ? round16<dtype>(p[8 * i + j]) : 0.0f;
     } else if (MODE == kNorm) {
       float w[8];
-      row8<dtype>(src.c, 8 * i, K, src.aligned, w);
+      if (i == tid) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = norm0[j];
+      } else {
+        row8<dtype>(src.c, 8 * i, K, src.aligned, w);
+      }
       const u32x4 r = xs[i];           // (the piece this thread wrote itself)
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(w[j] * (load16<dtype>((uint16_t)(r[j >> 1] >> (16 * (j & 1)))) * rs));
@@ -326,7 +366,7 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
       row8<dtype>(src.a, 8 * i, K, src.aligned, g);
       row8<dtype>(src.b, 8 * i, K, src.aligned, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(round16<dtype>(g[j] / (1.0f + expf(-g[j]))) * u[j]);
+      for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(round16<dtype>(silu(g[j])) * u[j]);
     } else {
       row8<dtype>(src.a, 8 * i, K, src.aligned, f);
     }
@@ -339,37 +379,59 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
     if (i % PPG == 0) sums[i / PPG] = s;
   }
   __syncthreads();
-  const int run = (n_tiles_k + WAVES - 1) / WAVES;
-  const int k_begin = min(wave * run, n_tiles_k), k_end = min(k_begin + run, n_tiles_k);
-  int buf = 0;
-  for (int tn = blockIdx.x; tn < n_tiles_n; tn += gridDim.x) {
-    float acc = 0.0f;
-    const u32x4 *tile = codes + (int64_t)tn * n_tiles_k * 64 + lane;
-    const uint32_t *words = scales + (int64_t)tn * n_tiles_k * GPC * 16 + n;
-    for (int kc = k_begin; kc < k_end; ++kc) {
-      const u32x4 q = load_stream(tile + (int64_t)kc * 64);
+  float acc = 0.0f;
+  int kept = 0;
+  auto flush = [&](int first) __attribute__((always_inline)) {      // `kept` tiles, from row tile `first` on
+    __syncthreads();
+    for (int i = tid; i < kept * 16; i += 64 * WAVES) {
+      const int64_t row = (int64_t)(first + (i >> 4) * (int)gridDim.x) * 16 + (i & 15);
+      if (row < N) {
+        float s = 0.0f;
 #pragma unroll
-      for (int g = 0; g < GPC; ++g) {
-        const uint32_t w = words[(kc * GPC + g) * 16];
-        f32x4 D = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int d = g * (4 / GPC); d < (g + 1) * (4 / GPC); ++d)
-          D = mfma<dtype>(xs[kc * 16 + 4 * d + c], operand<dtype>(q[d]), D);
-        acc = add_group<dtype>(w, D[0], sums[kc * GPC + g], acc);
+        for (int w = 0; w < WAVES; ++w) s += s_red[i >> 4][w][i & 15];
+        if (bias) s += load16<dtype>(bias[row]);
+        y[row] = bits16<dtype>(s);
       }
     }
-    // every lane of a column holds the same sum (all sixteen rows of the operand are the one row)
-    if (lane < 16) s_red[buf][wave][lane] = acc;
-    __syncthreads();
-    if (tid < 16 && tn * 16 + tid < N) {
-      float s = 0.0f;
+  };
+  auto compute = [&](Cur c, const Piece &p) __attribute__((always_inline)) {
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) s += s_red[buf][w][tid];
-      const int row = tn * 16 + tid;
-      if (bias) s += load16<dtype>(bias[row]);
-      y[row] = bits16<dtype>(s);
+    for (int u = 0; u < U; ++u) {
+      const int kc = k_begin + c.step * U + u;
+      if (kc < k_end) {
+#pragma unroll
+        for (int g = 0; g < GPC; ++g) {
+          f32x4 D = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int d = g * (4 / GPC); d < (g + 1) * (4 / GPC); ++d)
+            D = mfma<dtype>(xs[kc * 16 + 4 * d + quarter], operand<dtype>(p.q[u][d]), D);
+          acc = add_group<dtype>(p.w[u][g], D[0], sums[kc * GPC + g], acc);
+        }
+      }
     }
-    buf ^= 1;      // the next tile's sums go elsewhere: one barrier a tile
+    if (c.step + 1 == steps) {
+      // every lane of a column holds the same sum (all sixteen rows of the operand are the one row)
+      if (lane < 16) s_red[kept][wave][lane] = acc;
+      acc = 0.0f;
+      if (++kept == kKept) {
+        flush(c.tn - (kKept - 1) * (int)gridDim.x);
+        kept = 0;
+        __syncthreads();
+      }
+    }
+  };
+  while (ca.tn < n_tiles_n) {
+    const Cur cb = next(ca);
+    if (cb.tn < n_tiles_n) load(cb, pb);
+    compute(ca, pa);
+    if (cb.tn >= n_tiles_n) break;
+    ca = next(cb);
+    if (ca.tn < n_tiles_n) load(ca, pa);
+    compute(cb, pb);
+  }
+  if (kept) {
+    const int mine = (n_tiles_n - 1 - (int)blockIdx.x) / (int)gridDim.x;      // the workgroup's last tile
+    flush((int)blockIdx.x + (mine - kept + 1) * (int)gridDim.x);
   }
 }
 
@@ -384,20 +446,149 @@ w4_stage_rows_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_r
   out[m * K_padded + k] = k < K ? bits16<dtype>(rdkv_load_as_float(x, x_dtype, m * x_stride_row + k)) : (uint16_t)0;
 }
 
-// Several activation rows: MT tiles of 16 rows by NT row tiles of the weights a workgroup, its eight wavefronts
-// sharing the columns; the sums X come from a product with ones (all columns of it are X, where the lanes need it).
+// Two to sixteen activation rows: a workgroup takes a row tile of the weights (grid.x) and 16 activation rows (grid.y), its
+// wavefronts share the columns.  The rows' operands come straight from global memory (each is read by
+// one wavefront), the sums X from a product with ones (all columns of it are X, where the lanes need it).
 // x rows 16-byte aligned, K_x a multiple of 8 (what lies behind is taken as zero).
-template <int dtype, int GPC, int MT, int NT>
-__global__ void __launch_bounds__(512)
-w4_rows_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, const uint16_t *__restrict__ x,
-               int64_t x_stride_row, const uint16_t *__restrict__ bias, int M, int N, int K_x, int n_tiles_n,
-               int n_tiles_k, uint16_t *__restrict__ y, int64_t y_stride_row) {
-  extern __shared__ float s_acc[];      // [8][MT][NT][256]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane >> 4, n = lane & 15;
-  const int tn0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-  const uint16_t *rows[MT];
+template <int dtype, int GPC, int WAVES, int U>
+__global__ void __launch_bounds__(64 * WAVES)
+w4_few_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, const uint16_t *__restrict__ x,
+              int64_t x_stride_row, const uint16_t *__restrict__ bias, int M, int N, int K_x, int n_tiles_k,
+              uint16_t *__restrict__ y, int64_t y_stride_row) {
+  __shared__ float s_acc[WAVES][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 4, n = lane & 15;
+  const int tn = blockIdx.x, m0 = blockIdx.y * 16;
+  const uint16_t *row = x + (int64_t)min(m0 + n, M - 1) * x_stride_row;
+  const u32x4 *tile = codes + (int64_t)tn * n_tiles_k * 64 + lane;
+  const uint32_t *words = scales + (int64_t)tn * n_tiles_k * GPC * 16 + n;
+  constexpr uint32_t one2 = dtype == RDKV_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
+  const u32x4 ones = {one2, one2, one2, one2};
+  struct Piece { u32x4 q[U], a[U][4]; uint32_t w[U][GPC]; };
+  const int run = (n_tiles_k + WAVES - 1) / WAVES, k_begin = min(wave * run, n_tiles_k), k_end = min(k_begin + run, n_tiles_k);
+  auto load = [&](int k0, Piece &p) __attribute__((always_inline)) {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) rows[mt] = x + (int64_t)min(m0 + 16 * mt + n, M - 1) * x_stride_row + 8 * c;
+    for (int u = 0; u < U; ++u) {
+      const int kc = k0 + u < k_end ? k0 + u : k0;
+      p.q[u] = load_stream(tile + (int64_t)kc * 64);
+#pragma unroll
+      for (int g = 0; g < GPC; ++g) p.w[u][g] = words[(kc * GPC + g) * 16];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int k = kc * kTileCols + 32 * d + 8 * c;
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + (k < K_x ? k : 0));
+        p.a[u][d] = k < K_x ? v : u32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](int k0, const Piece &p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u < k_end) {
+#pragma unroll
+        for (int g = 0; g < GPC; ++g) {
+          f32x4 D = {0.0f, 0.0f, 0.0f, 0.0f}, X = D;
+#pragma unroll
+          for (int d = g * (4 / GPC); d < (g + 1) * (4 / GPC); ++d) {
+            D = mfma<dtype>(p.a[u][d], operand<dtype>(p.q[u][d]), D);
+            X = mfma<dtype>(p.a[u][d], ones, X);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = add_group<dtype>(p.w[u][g], D[i], X[i], acc[i]);
+        }
+      }
+    }
+  };
+  Piece pa, pb;
+  int k0 = k_begin;
+  if (k0 < k_end) load(k0, pa);
+  while (k0 < k_end) {
+    if (k0 + U < k_end) load(k0 + U, pb);
+    compute(k0, pa);
+    k0 += U;
+    if (k0 >= k_end) break;
+    if (k0 + U < k_end) load(k0 + U, pa);
+    compute(k0, pb);
+    k0 += U;
+  }
+  // register i of lane 16 c + n: activation row 4 c + i, weight row n
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s_acc[wave][(4 * c + i) * 16 + n] = acc[i];
+  __syncthreads();
+  if (tid < 256) {
+    const int m = m0 + (tid >> 4), r = tn * 16 + (tid & 15);
+    if (m < M && r < N) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += s_acc[w][tid];
+      if (bias) s += load16<dtype>(bias[r]);
+      y[(int64_t)m * y_stride_row + r] = bits16<dtype>(s);
+    }
+  }
+}
+
+// More rows.  A first launch lays the activations out in operand order, sixteen rows by a column tile at a time (piece p,
+// columns 8 p .. 8 p + 7, of row m at 16-byte slot 16 p + m: what lane 16 c + m reads for p = 4 d + c), zeros behind the
+// matrix, and forms the sums X; every workgroup of the second launch then copies whole blocks.  Blocks follow each other by
+// column tile within MT tiles of rows: the operands of the MT tiles, then their sums [group][row].
+template <int dtype>
+__device__ __forceinline__ float sum8(u32x4 v) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = v[i];
+    s += load16<dtype>((uint16_t)pair);
+    s += load16<dtype>((uint16_t)(pair >> 16));
+  }
+  return s;
+}
+template <int GPC, int MT>
+struct Block { u32x4 x[MT * 256]; float sum[GPC][16 * MT]; };
+
+template <int dtype, int GPC, int MT>
+__global__ void __launch_bounds__(256)
+w4_blocks_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_row, int aligned, int M, int K,
+                 Block<GPC, MT> *__restrict__ out) {
+  const int tid = threadIdx.x, piece = tid & 15, m = tid >> 4;
+  const int kc = blockIdx.x, mt = blockIdx.y % MT;
+  const int64_t row = (int64_t)blockIdx.y * 16 + m;
+  Block<GPC, MT> &block = out[(int64_t)(blockIdx.y / MT) * gridDim.x + kc];
+  const int k = kc * kTileCols + 8 * piece;
+  u32x4 v = {0, 0, 0, 0};
+  if (row < M) {
+    if (aligned && k + 8 <= K) {
+      v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(x) + row * x_stride_row + k);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = k + j < K ? rdkv_load_as_float(x, x_dtype, row * x_stride_row + k + j) : 0.0f;
+      v = pack8<dtype>(f);
+    }
+  }
+  block.x[mt * 256 + piece * 16 + m] = v;
+  float s = sum8<dtype>(v);
+  s += rdkv_dpp_mov<0xB1>(s);                    // lanes of a pair, of four, of eight, of sixteen
+  s += rdkv_dpp_mov<0x4E>(s);
+  if (GPC <= 2) s += rdkv_dpp_mov<0x141>(s);
+  if (GPC == 1) s += rdkv_dpp_mov<0x140>(s);
+  if (piece % (16 / GPC) == 0) block.sum[piece / (16 / GPC)][16 * mt + m] = s;
+}
+
+// A workgroup takes 16 MT activation rows by 128 rows of the weights.  Two sets of four wavefronts take the column tiles in
+// turn (even, odd); a set copies the next block to LDS while it computes on the one before.  A wavefront multiplies it
+// with two row tiles of the weights.
+template <int dtype, int GPC, int MT>
+__global__ void __launch_bounds__(512)
+w4_tile_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, const Block<GPC, MT> *__restrict__ blocks,
+               const uint16_t *__restrict__ bias, int M, int N, int n_tiles_n, int n_tiles_k, uint16_t *__restrict__ y,
+               int64_t y_stride_row) {
+  constexpr int NT = 2, kSums = GPC * 16 * MT;
+  static_assert(kSums <= 256, "a set's threads copy one sum each");
+  __shared__ Block<GPC, MT> s_block[2][2];        // [set][buffer]
+  const int tid = threadIdx.x, lane = tid & 63, set = __builtin_amdgcn_readfirstlane(tid >> 8),
+            wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane >> 4, n = lane & 15, st = tid & 255;
+  const int tn0 = blockIdx.x * 8 + wave * NT, m0 = blockIdx.y * (16 * MT);
+  const Block<GPC, MT> *from = blocks + (int64_t)blockIdx.y * n_tiles_k;
   const u32x4 *tile[NT];
   const uint32_t *words[NT];
 #pragma unroll
@@ -406,73 +597,115 @@ w4_rows_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ sca
     tile[nt] = codes + tn * n_tiles_k * 64 + lane;
     words[nt] = scales + tn * n_tiles_k * GPC * 16 + n;
   }
-  f32x4 acc[MT][NT];
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr uint32_t one2 = dtype == RDKV_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
-  const u32x4 ones = {one2, one2, one2, one2};
-  for (int kc = wave; kc < n_tiles_k; kc += 8) {
-    u32x4 q[NT];
+    for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  struct Weights { u32x4 q[NT]; uint32_t w[NT][GPC]; };
+  struct Copy { u32x4 x[MT]; float sum; };
+  auto load_x = [&](int kc, Copy &v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) q[nt] = tile[nt][(int64_t)kc * 64];
-    u32x4 a[MT][4];
+    for (int j = 0; j < MT; ++j) v.x[j] = from[kc].x[256 * j + st];
+    v.sum = (&from[kc].sum[0][0])[min(st, kSums - 1)];
+  };
+  auto store_x = [&](Block<GPC, MT> &to, const Copy &v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int j = 0; j < MT; ++j) to.x[256 * j + st] = v.x[j];
+    if (st < kSums) (&to.sum[0][0])[st] = v.sum;
+  };
+  auto load_w = [&](int kc, Weights &w) __attribute__((always_inline)) {
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int k = kc * kTileCols + 32 * d;
-        const bool in = k + 8 * c < K_x;
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(rows[mt] + (in ? k : -8 * c));   // (else the row's start)
-        a[mt][d] = in ? v : u32x4{0, 0, 0, 0};
+    for (int nt = 0; nt < NT; ++nt) {
+      w.q[nt] = tile[nt][(int64_t)kc * 64];
+#pragma unroll
+      for (int g = 0; g < GPC; ++g) w.w[nt][g] = words[nt][(kc * GPC + g) * 16];
+    }
+  };
+  // The operands of the next 32 columns are read from LDS while the matrix cores work on the current ones.
+  auto compute = [&](const Block<GPC, MT> &b, const Weights &w) __attribute__((always_inline)) {
+    u32x4 a[2][MT];
+    f32x4 D[NT][MT], X[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) a[0][mt] = b.x[mt * 256 + lane];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      constexpr int DPG = 4 / GPC;
+      if (d + 1 < 4) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) a[(d + 1) & 1][mt] = b.x[mt * 256 + (d + 1) * 64 + lane];
       }
+      if ((d + 1) % DPG == 0) {
 #pragma unroll
-    for (int g = 0; g < GPC; ++g) {
-      f32x4 X[MT];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        X[mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int d = g * (4 / GPC); d < (g + 1) * (4 / GPC); ++d) X[mt] = mfma<dtype>(a[mt][d], ones, X[mt]);
+        for (int mt = 0; mt < MT; ++mt) X[mt] = *reinterpret_cast<const f32x4 *>(&b.sum[d / DPG][16 * mt + 4 * c]);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t w = words[nt][(kc * GPC + g) * 16];
-        f32x4 D[MT];
+        const u32x4 o = operand<dtype>(w.q[nt][d]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) D[mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int mt = 0; mt < MT; ++mt) D[nt][mt] = mfma<dtype>(a[d & 1][mt], o, d % DPG == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : D[nt][mt]);
+      }
+      if ((d + 1) % DPG == 0) {
 #pragma unroll
-        for (int d = g * (4 / GPC); d < (g + 1) * (4 / GPC); ++d) {
-          const u32x4 b = operand<dtype>(q[nt][d]);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) D[mt] = mfma<dtype>(a[mt][d], b, D[mt]);
-        }
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int i = 0; i < 4; ++i)
+              acc[nt][mt][i] = add_group<dtype>(w.w[nt][d / DPG], D[nt][mt][i], X[mt][i], acc[nt][mt][i]);
+      }
+    }
+  };
+  // Both sets make the same number of steps.  The loads of a step are issued two steps ahead (behind the last tile: the
+  // last one again, not used; without a branch, so that a wait leaves the younger loads in flight).
+  const int steps = (n_tiles_k + 1) / 2;
+  auto at = [&](int step) __attribute__((always_inline)) { return min(2 * step + set, n_tiles_k - 1); };
+  Weights w[2];
+  Copy xv[2];
+  load_x(at(0), xv[0]);
+  load_w(at(0), w[0]);
+  load_x(at(1), xv[1]);
+  load_w(at(1), w[1]);
+  store_x(s_block[set][0], xv[0]);
+  __syncthreads();
+  for (int step0 = 0; step0 < steps; step0 += 2) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[mt][nt][i] = add_group<dtype>(w, D[mt][i], X[mt][i], acc[mt][nt][i]);
+    for (int j = 0; j < 2; ++j) {
+      const int step = step0 + j;
+      if (step < steps) {
+        load_x(at(step + 2), xv[j]);
+        if (2 * step + set < n_tiles_k) compute(s_block[set][j], w[j]);
+        load_w(at(step + 2), w[j]);
+        store_x(s_block[set][j ^ 1], xv[j ^ 1]);
+        __syncthreads();
       }
     }
   }
-  // register i of lane 16 c + n: activation row 4 c + i, weight row n
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  // the odd set's sums join the even one's (all reads of the blocks are behind the barrier)
+  static_assert(sizeof(s_block) >= 4 * NT * MT * 256 * 4, "the sums of a set fit the blocks");
+  f32x4 *join = reinterpret_cast<f32x4 *>(&s_block[0][0]) + wave * (NT * MT * 64) + lane;
+  if (set == 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s_acc[((wave * MT + mt) * NT + nt) * 256 + (4 * c + i) * 16 + n] = acc[mt][nt][i];
+      for (int mt = 0; mt < MT; ++mt) join[(nt * MT + mt) * 64] = acc[nt][mt];
+  }
   __syncthreads();
-  for (int e = tid; e < MT * NT * 256; e += 512) {
-    const int in_tile = e & 255, nt = (e >> 8) % NT, mt = (e >> 8) / NT;
-    const int m = m0 + 16 * mt + (in_tile >> 4);
-    const int64_t row = (int64_t)(tn0 + nt) * 16 + (in_tile & 15);
-    if (m >= M || row >= N) continue;
-    float s = 0.0f;
+  if (set == 1) return;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += s_acc[w * (MT * NT * 256) + e];
-    if (bias) s += load16<dtype>(bias[row]);
-    y[(int64_t)m * y_stride_row + row] = bits16<dtype>(s);
+  for (int nt = 0; nt < NT; ++nt) {
+    const int64_t r = (int64_t)(tn0 + nt) * 16 + n;
+    const float b = bias && r < N ? load16<dtype>(bias[r]) : 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const f32x4 other = join[(nt * MT + mt) * 64];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = m0 + 16 * mt + 4 * c + i;
+        if (m < M && r < N) y[(int64_t)m * y_stride_row + r] = bits16<dtype>(acc[nt][mt][i] + other[i] + b);
+      }
+    }
   }
 }
 
@@ -511,11 +744,11 @@ bool aligned16(const void *p) { return ((uintptr_t)p % 16) == 0; }
 template <int dtype, int MODE, int GPC>
 void launch_row(const Shape &sh, const void *codes, const uint32_t *scales, const RowSource &src, const void *bias, int N,
                 int K, void *y, hipStream_t s) {
-  constexpr int WAVES = 8;
+  constexpr int WAVES = 16, U = 2;
   const int cus = compute_units();
   const size_t lds = (size_t)sh.n_tiles_k * (256 + 4 * GPC);
   const int grid = sh.n_tiles_n < 2 * cus ? sh.n_tiles_n : 2 * cus;
-  hipLaunchKernelGGL((w4_row_kernel<dtype, MODE, GPC, WAVES>), dim3(grid), dim3(64 * WAVES), lds, s, (const u32x4 *)codes,
+  hipLaunchKernelGGL((w4_row_kernel<dtype, MODE, GPC, WAVES, U>), dim3(grid), dim3(64 * WAVES), lds, s, (const u32x4 *)codes,
                      scales, src, (const uint16_t *)bias, N, K, sh.n_tiles_n, sh.n_tiles_k, (uint16_t *)y);
 }
 template <int MODE>
@@ -532,19 +765,47 @@ void launch_row_any(int dtype, const Shape &sh, const void *codes, const uint32_
 #undef RDKV_W4_ROW
 }
 
-struct Rows { const uint16_t *x; int64_t x_stride; int K_x; const uint16_t *bias; int M, N; uint16_t *y; int64_t y_stride; };
-template <int dtype, int GPC, int MT, int NT>
-void launch_rows(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
-  const dim3 grid((unsigned)rdkv_cdiv(sh.n_tiles_n, NT), (unsigned)rdkv_cdiv(r.M, 16 * MT));
-  hipLaunchKernelGGL((w4_rows_kernel<dtype, GPC, MT, NT>), grid, dim3(512), (size_t)8 * MT * NT * 1024, s,
-                     (const u32x4 *)codes, scales, r.x, r.x_stride, r.bias, r.M, r.N, r.K_x, sh.n_tiles_n, sh.n_tiles_k,
-                     r.y, r.y_stride);
+struct Rows {
+  const void *x;
+  int x_dtype;
+  int64_t x_stride;
+  int aligned;                 // rows of the weights' type that can be read in 16-byte pieces
+  int K;
+  const uint16_t *bias;
+  int M, N;
+  uint16_t *y;
+  int64_t y_stride;
+  void *workspace;
+};
+template <int dtype, int GPC, int MT>
+void launch_tile(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
+  const unsigned blocks = (unsigned)rdkv_cdiv(r.M, 16 * MT);
+  auto *at = reinterpret_cast<Block<GPC, MT> *>(r.workspace);
+  hipLaunchKernelGGL((w4_blocks_kernel<dtype, GPC, MT>), dim3(sh.n_tiles_k, blocks * MT), dim3(256), 0, s, r.x, r.x_dtype, r.x_stride,
+                     r.aligned, r.M, r.K, at);
+  hipLaunchKernelGGL((w4_tile_kernel<dtype, GPC, MT>), dim3((unsigned)rdkv_cdiv(sh.n_tiles_n, 8), blocks), dim3(512), 0, s,
+                     (const u32x4 *)codes, scales, at, r.bias, r.M, r.N, sh.n_tiles_n, sh.n_tiles_k, r.y, r.y_stride);
 }
 template <int dtype, int GPC>
-void launch_rows_any(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
-  if (r.M <= 16) launch_rows<dtype, GPC, 1, 1>(sh, codes, scales, r, s);
-  else if (r.M <= 32) launch_rows<dtype, GPC, 2, 1>(sh, codes, scales, r, s);
-  else launch_rows<dtype, GPC, 4, 1>(sh, codes, scales, r, s);
+void launch_few(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
+  const uint16_t *x = (const uint16_t *)r.x;
+  int64_t stride = r.x_stride;
+  int K_x = r.K;
+  if (!r.aligned) {            // a padded copy first
+    K_x = sh.n_tiles_k * kTileCols;
+    stride = K_x;
+    x = (const uint16_t *)r.workspace;
+    hipLaunchKernelGGL(w4_stage_rows_kernel<dtype>, dim3((unsigned)rdkv_cdiv(K_x, 256), r.M), dim3(256), 0, s, r.x, r.x_dtype, r.x_stride,
+                       r.K, K_x, (uint16_t *)r.workspace);
+  }
+  hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 16, 2>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(1024), 0, s,
+                     (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K_x, sh.n_tiles_k, r.y, r.y_stride);
+}
+template <int dtype, int GPC>
+void launch_rows(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
+  if (r.M <= 16) launch_few<dtype, GPC>(sh, codes, scales, r, s);
+  else if (r.M <= 32) launch_tile<dtype, GPC, 2>(sh, codes, scales, r, s);
+  else launch_tile<dtype, GPC, 4>(sh, codes, scales, r, s);
 }
 
 }  // namespace
@@ -635,7 +896,10 @@ RDKV_API int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, i
 
 RDKV_API int64_t rdkv_w4_linear_workspace_bytes(int M, int K) {
   if (M <= 0 || K <= 0) return 0;
-  return (int64_t)M * rdkv_cdiv(K, kTileCols) * kTileCols * 2;
+  const int64_t n_tiles_k = rdkv_cdiv(K, kTileCols);
+  if (M <= 16) return M * n_tiles_k * kTileCols * 2;
+  // whole blocks of 32 or 64 rows, their sums at the finest groups
+  return rdkv_cdiv(M, M <= 32 ? 32 : 64) * n_tiles_k * (int64_t)(M <= 32 ? sizeof(Block<4, 2>) : sizeof(Block<4, 4>));
 }
 
 RDKV_API int rdkv_w4_linear(const void *codes, const uint32_t *scales, const void *x, int x_dtype, int64_t x_stride_row,
@@ -645,7 +909,7 @@ RDKV_API int rdkv_w4_linear(const void *codes, const uint32_t *scales, const voi
   Shape sh;
   const int rc = check_shape(fn, N, K, group, dtype, &sh);
   if (rc != RDKV_OK) return rc;
-  RDKV_REQUIRE(M >= 0 && M <= 65535 * 16, "%s: %d rows", fn, M);
+  RDKV_REQUIRE(M >= 0 && M <= 1 << 20, "%s: %d rows", fn, M);
   if (N == 0 || M == 0) return RDKV_OK;
   RDKV_REQUIRE(codes && scales && x && y && aligned16(codes), "%s: null or misaligned pointer", fn);
   RDKV_REQUIRE(x_dtype == dtype || x_dtype == RDKV_DTYPE_F32, "%s: x must have the weights' type or be fp32", fn);
@@ -658,34 +922,20 @@ RDKV_API int rdkv_w4_linear(const void *codes, const uint32_t *scales, const voi
     RDKV_CHECK_LAUNCH(fn);
     return RDKV_OK;
   }
-  Rows r = {(const uint16_t *)x, x_stride_row, K, (const uint16_t *)bias, M, N, (uint16_t *)y, y_stride_row};
-  if (x_dtype != dtype || !aligned16(x) || (M > 1 && x_stride_row % 8 != 0) || K % 8 != 0) {
-    // rows that cannot be read in 16-byte pieces (or are fp32): a padded copy first
-    const int K_padded = sh.n_tiles_k * kTileCols;
-    if (!workspace || workspace_bytes < rdkv_w4_linear_workspace_bytes(M, K) || !aligned16(workspace)) {
-      rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)rdkv_w4_linear_workspace_bytes(M, K));
+  const int aligned = x_dtype == dtype && aligned16(x) && (M == 1 || x_stride_row % 8 == 0) && K % 8 == 0;
+  if (M > 16 || !aligned) {
+    const int64_t need = rdkv_w4_linear_workspace_bytes(M, K);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace)) {
+      rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
       return RDKV_EWORKSPACE;
     }
-    // (a grid's second dimension takes 65535 rows)
-    for (int64_t m = 0; m < M; m += 65535) {
-      const dim3 grid((unsigned)rdkv_cdiv(K_padded, 256), (unsigned)(M - m < 65535 ? M - m : 65535));
-      const char *from = (const char *)x + m * x_stride_row * (x_dtype == RDKV_DTYPE_F32 ? 4 : 2);
-      uint16_t *to = (uint16_t *)workspace + m * K_padded;
-      if (dtype == RDKV_DTYPE_F16)
-        hipLaunchKernelGGL(w4_stage_rows_kernel<RDKV_DTYPE_F16>, grid, dim3(256), 0, s, from, x_dtype, x_stride_row, K, K_padded, to);
-      else
-        hipLaunchKernelGGL(w4_stage_rows_kernel<RDKV_DTYPE_BF16>, grid, dim3(256), 0, s, from, x_dtype, x_stride_row, K, K_padded, to);
-      RDKV_CHECK_LAUNCH(fn);
-    }
-    r.x = (const uint16_t *)workspace;
-    r.x_stride = K_padded;
-    r.K_x = K_padded;
   }
-#define RDKV_W4_ROWS(DT)                                                  \
-  do {                                                                    \
-    if (sh.gpc == 1) launch_rows_any<DT, 1>(sh, codes, scales, r, s);     \
-    else if (sh.gpc == 2) launch_rows_any<DT, 2>(sh, codes, scales, r, s); \
-    else launch_rows_any<DT, 4>(sh, codes, scales, r, s);                 \
+  const Rows r = {x, x_dtype, x_stride_row, aligned, K, (const uint16_t *)bias, M, N, (uint16_t *)y, y_stride_row, workspace};
+#define RDKV_W4_ROWS(DT)                                              \
+  do {                                                                \
+    if (sh.gpc == 1) launch_rows<DT, 1>(sh, codes, scales, r, s);     \
+    else if (sh.gpc == 2) launch_rows<DT, 2>(sh, codes, scales, r, s); \
+    else launch_rows<DT, 4>(sh, codes, scales, r, s);                 \
   } while (0)
   if (dtype == RDKV_DTYPE_F16) RDKV_W4_ROWS(RDKV_DTYPE_F16);
   else RDKV_W4_ROWS(RDKV_DTYPE_BF16);
