@@ -12,8 +12,8 @@
 //
 // Three launches.  Maximum: the slices of a row leave their largest logit and its place.  Histogram: sums (and, under top-k,
 // counts) of the weights in bins of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup
-// per row adds the bins up, finds a search's bin, collects the bin's tokens from the row and resolves them, by
-// further bins over (logit, index) while they are many.
+// per row adds the bins up, which tells in which bins the searches can end, collects those bins' tokens in one pass over the
+// row and resolves the searches among them, by further bins over (logit, index) while they are many.
 #include "rdkv_common.h"
 #include "rope_device.h"
 
@@ -24,7 +24,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kOctaves = 46, kPerOctave = 32, kBins = kOctaves * kPerOctave;
 constexpr int kMaxSlices = 64;
 constexpr int kMaxVocab = 1 << 24;
-constexpr int kList = 2048;              // tokens of a bin that LDS holds
 
 // Workspace of a row: the slices' maxima, then the histogram.
 struct RowSpace {
@@ -61,27 +60,33 @@ __device__ __forceinline__ uint64_t composite(float l, int index) {
 __device__ __forceinline__ float composite_logit(uint64_t c) { return rdkv_ordered_to_float((uint32_t)(c >> 32)); }
 __device__ __forceinline__ int composite_index(uint64_t c) { return (int)~(uint32_t)c; }
 
-// Octaves below the maximum, in fp64; bin and weight of a token.  Two launches form them and add them up to the same
-// sums, bit for bit: nothing is contracted that is not written as fma.
-struct Scale { float m; double inv; int top; };     // maximum, log2(e) / T, weight 2^top of the maximum
-__device__ __forceinline__ double octaves(const Scale &s, float l) {
+// Bins below the maximum, in fp64 (the bin, and the place in it), and the weight there.  Two launches form them and add
+// them up to the same sums, bit for bit: nothing is contracted that is not written as fma.
+struct Scale { float m; double inv; int top; };     // maximum, bins per unit of logit, weight 2^top of the maximum
+__device__ __forceinline__ Scale scale_of(uint64_t best, float T, int top) {
+  return Scale{rdkv_ordered_to_float((uint32_t)(best >> 32)), 1.44269504088896340736 * kPerOctave / (double)T, top};
+}
+__device__ __forceinline__ double bins_below(const Scale &s, float l) {
 #pragma clang fp contract(off)
   return l == s.m ? 0.0 : ((double)s.m - (double)l) * s.inv;
 }
-// 2^-t as an integer: 2^-(bin / 32) from the table, the rest by its series (within 2e-13)
+// 2^(top - t / 32) as an integer: 2^(52 - i / 32) of the bin's place in its octave from the table, times the series of
+// 2^(-f / 32) for the rest f < 1 (2e-13 of it left out), added to 2^52 for its bits as an integer, shifted.
 __device__ __forceinline__ uint64_t weight(const Scale &s, const double *table, double t) {
 #pragma clang fp contract(off)
-  const int bin = (int)(t * kPerOctave);
-  const double y = (t - bin * (1.0 / kPerOctave)) * 0.693147180559945309417;
-  double p = fma(y, -1.0 / 120, 1.0 / 24);
-  p = fma(y, p, -1.0 / 6);
-  p = fma(y, p, 0.5);
-  p = fma(y, p, -1.0);
-  p = fma(y, p, 1.0) * table[bin & (kPerOctave - 1)];
-  return (uint64_t)ldexp(p, s.top - (bin >> 5));
+  constexpr double a = 0.693147180559945309417 / kPerOctave;
+  const int bin = (int)t;
+  const double f = __builtin_amdgcn_fract(t);
+  double p = fma(f, -a * a * a * a * a / 120, a * a * a * a / 24);
+  p = fma(f, p, -a * a * a / 6);
+  p = fma(f, p, a * a / 2);
+  p = fma(f, p, -a);
+  p = fma(f, p, 1.0);
+  const double sum = fma(p, table[bin & (kPerOctave - 1)], 0x1p52);
+  return (__builtin_bit_cast(uint64_t, sum) - 0x4330000000000000ull) >> (52 - s.top + (bin >> 5));
 }
 __device__ __forceinline__ void fill_table(double *table) {
-  if (threadIdx.x < kPerOctave) table[threadIdx.x] = exp2(-(double)threadIdx.x / kPerOctave);
+  if (threadIdx.x < kPerOctave) table[threadIdx.x] = exp2(52.0 - (double)threadIdx.x / kPerOctave);
 }
 
 template <int dtype>
@@ -136,6 +141,8 @@ struct Row {
   }
 };
 
+__device__ __forceinline__ uint64_t lesser(uint64_t a, uint64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -198,19 +205,21 @@ sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, i
   }
   if (tid == 0) s_least = 0;
   __syncthreads();
-  const Scale sc = {composite_logit(best), 1.44269504088896340736 / (double)set.T, top};
-  const double least_w = (double)set.min_p * ldexp(1.0, top);
+  const Scale sc = scale_of(best, set.T, top);
+  // w >= min_p as bins below the maximum; without top-p nobody asks about what lies beyond
+  const double least_t = least ? -log2((double)fminf(set.min_p, 1.0f)) * kPerOctave : 0.0;
+  const double need = least && !(set.top_p < 1.0f) ? fmin(least_t + 1.0, (double)kBins) : (double)kBins;
   const Row<dtype> row(logits, stride, blockIdx.y, vocab);
   const int per = (row.pieces + slices - 1) / slices, begin = min(slice * per, row.pieces), end = min(begin + per, row.pieces);
   uint64_t least_mass = 0;
   row.template each<256>(begin, end, slice == 0, [&](float l, int i, bool there) __attribute__((always_inline)) {
-    const double t = octaves(sc, l);
-    if (there && l > -INFINITY && t < (double)kOctaves) {
+    const double t = bins_below(sc, l);
+    if (there && l > -INFINITY && t < need) {
       const uint64_t w = weight(sc, s_table, t);
-      const int bin = (int)(t * kPerOctave);
+      const int bin = (int)t;
       atomicAdd((unsigned long long *)&s_mass[bin], (unsigned long long)w);
       if (counts) atomicAdd(&s_count[bin], 1u);
-      if (least && (double)w >= least_w) least_mass += w;
+      if (least && t <= least_t) least_mass += w;
     }
   });
   if (least && least_mass) atomicAdd((unsigned long long *)&s_least, (unsigned long long)least_mass);
@@ -232,201 +241,184 @@ struct Advance {                         // rdkv_argmax_advance's counters, of a
   int n_uniform;
 };
 
+constexpr int kList = 4096;              // tokens that the last launch sorts, and pieces that it looks into
+
 struct Choice {                          // LDS of the last launch
-  uint64_t mass[kBins + 1];              // sums in front of a bin, the whole sum at the end
+  uint64_t mass[kBins + 1];              // sums (counts) in front of a bin, the whole at the end
   uint32_t count[kBins + 1];
-  uint64_t sub_mass[1024];
-  uint32_t sub_count[1024];
-  uint64_t list[2][kList];
+  uint64_t list[kList];                  // the tokens of the searches' bins; sorted, with the sum in front of each and
+  uint64_t before[kList], own[kList];    // its own weight
+  union {
+    uint32_t pieces[kList];              // pieces of the row that may hold one
+    struct {                             // of the sorted list, where a bin's run starts: its sum and its place
+      uint64_t run_mass[kBins];
+      uint32_t run_at[kBins];
+    };
+    struct {                             // further bins of the pass for crowded rows
+      uint64_t sub_mass[1024];
+      uint32_t sub_count[1024];
+    };
+  };
   uint64_t part_mass[16];
   uint32_t part_count[16];
   double table[kPerOctave];
   uint64_t lo, hi, found, upto;
-  int bin, n;
+  int bin[5], n_pieces, n;
 };
 
-// Sums in front of each of N entries (N at most 2048: two a thread), in place; [N] takes the whole.
-template <int N>
-__device__ __forceinline__ void prefix(uint64_t *mass, uint32_t *count, Choice &s) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int i0 = 2 * tid, i1 = i0 + 1;
-  uint64_t m0 = i0 < N ? mass[i0] : 0, m1 = i1 < N ? mass[i1] : 0;
-  uint32_t c0 = i0 < N ? count[i0] : 0, c1 = i1 < N ? count[i1] : 0;
-  uint64_t m = m0 + m1;
-  uint32_t c = c0 + c1;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t um = __shfl_up(m, o, 64);
-    const uint32_t uc = __shfl_up(c, o, 64);
-    if (lane >= o) {
-      m += um;
-      c += uc;
-    }
-  }
-  if (lane == 63) {
-    s.part_mass[wave] = m;
-    s.part_count[wave] = c;
+// Inclusive sums over the lanes of a wavefront (shifts inside rows of sixteen, then the rows' last lanes handed on).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved64(uint64_t v) {
+  return ((uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | moved<CTRL, ROWS>((uint32_t)v);
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v += moved64<0x111, 0xf>(v);
+  v += moved64<0x112, 0xf>(v);
+  v += moved64<0x114, 0xf>(v);
+  v += moved64<0x118, 0xf>(v);
+  v += moved64<0x142, 0xa>(v);
+  return v + moved64<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  return v + moved<0x143, 0xc>(v);
+}
+// Sums over the workgroup's threads in front of this one.
+__device__ __forceinline__ void block_scan(Choice &s, uint64_t &m, uint32_t &c) {
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const uint64_t sm = wave_scan(m);
+  const uint32_t sc = wave_scan(c);
+  if ((tid & 63) == 63) {
+    s.part_mass[wave] = sm;
+    s.part_count[wave] = sc;
   }
   __syncthreads();
-  uint64_t bm = m - m0 - m1;
-  uint32_t bc = c - c0 - c1;
+  uint64_t bm = sm - m;
+  uint32_t bc = sc - c;
   for (int w = 0; w < wave; ++w) {
     bm += s.part_mass[w];
     bc += s.part_count[w];
   }
-  if (i0 < N) { mass[i0] = bm; count[i0] = bc; }
-  if (i1 < N) { mass[i1] = bm + m0; count[i1] = bc + c0; }
   __syncthreads();
+  m = bm;
+  c = bc;
 }
 
-// The first token, in the tokens' order, whose running count (by_count) or sum exceeds `target`, and the sum up to and
-// with it; the bins' own totals exceed the target.  All threads of the workgroup take part.
+// Puts v into the list of every lane whose `in` holds (the whole wavefront takes part); *n counts them all.
+template <class T>
+__device__ __forceinline__ void append(T *list, int *n, bool in, T v) {
+  const uint64_t mask = __ballot(in);
+  if (mask == 0) return;
+  const int lane = threadIdx.x & 63, first = __ffsll((unsigned long long)mask) - 1;
+  int at = 0;
+  if (lane == first) at = atomicAdd(n, __popcll(mask));
+  at = __shfl(at, first, 64) + __popcll(mask & ((1ull << lane) - 1));
+  if (in && at < kList) list[at] = v;
+}
+
+// Logits that can lie in bins [from, to] as a distance from a middle, wide enough for every rounding on the way; what is
+// found is tested exactly.
+struct Near { float middle, half; };
+__device__ __forceinline__ Near near_bins(const Scale &sc, float T, int from, int to) {
+  const double w = (double)T * (0.693147180559945309417 / kPerOctave);      // logits a bin
+  const double lo = (double)sc.m - ((double)to + 1.001) * w, hi = (double)sc.m - ((double)from - 0.001) * w;
+  Near n = {(float)(0.5 * (lo + hi)), (float)(0.5 * (hi - lo))};
+  n.half += n.half * 0x1p-20f + fabsf(n.middle) * 0x1p-22f;
+  if (!(fabsf(n.middle) < INFINITY) || !(n.half < INFINITY)) n = Near{0.0f, INFINITY};
+  return n;
+}
+
+// Targets of the questions.
+__device__ __forceinline__ uint64_t top_p_target(float top_p, uint64_t kept) {
+  const double want = ceil((double)top_p * (double)kept);
+  const uint64_t target = want >= 1.0 ? (uint64_t)want - 1 : 0;
+  return target < kept ? target : kept - 1;
+}
+__device__ __forceinline__ uint64_t token_target(float u, uint64_t run) {
+  const double x = (double)u * (double)run;
+  const uint64_t target = x > 0.0 ? (x < (double)run ? (uint64_t)x : run - 1) : 0;
+  return target < run ? target : run - 1;
+}
+
+// Crowded rows (thousands of tokens in the bins of a search: flat rows, equal logits): the first token of `bin` whose running
+// count or sum, from the bin's start on, exceeds `target`, by 1024 further bins at a time over the composites of the
+// tokens in question, each from a pass over the row.  Composites are distinct and a round leaves at most a 512th of
+// their range, so a handful of rounds end at one token.
 template <int dtype>
-__device__ void search(Choice &s, const Row<dtype> &row, const Scale &sc, bool by_count, uint64_t target) {
-  const int tid = threadIdx.x;
-  for (int i = tid; i < kBins; i += 1024) {
-    const uint64_t a = by_count ? s.count[i] : s.mass[i], b = by_count ? s.count[i + 1] : s.mass[i + 1];
-    if (a <= target && target < b) s.bin = i;            // (one bin only)
-  }
-  if (tid == 0) {
-    s.n = 0;
-    s.lo = ~0ull;
-    s.hi = 0;
-  }
-  __syncthreads();
-  const int bin = s.bin;
-  uint64_t base = s.mass[bin];
-  target -= by_count ? s.count[bin] : base;
-  // the bin's tokens: a cheap test in fp32 (a thousandth of a bin off at most) in front of the exact one
-  const float inv32 = (float)(sc.inv * kPerOctave), from = bin - 0.1f, to = bin + 1.1f;
-  // (not where the factor leaves fp32, or a difference could that is fewer than 46 octaves)
-  const bool coarse = sc.inv < 1e30 && sc.inv > 1e-30;
-  const int lane = tid & 63;
-  auto in_bin = [&](float l, bool there) __attribute__((always_inline)) {
-    if (!there || !(l > -INFINITY)) return false;
-    const float tf = (sc.m - l) * inv32;
-    if (coarse && (tf < from || tf > to)) return false;
-    const double t = octaves(sc, l);
-    return t < (double)kOctaves && (int)(t * kPerOctave) == bin;
+__device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row, const Scale &sc, int bin, bool by_count,
+                                               uint64_t target) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t base = s.mass[bin], from = 0, to = ~0ull;
+  auto each_in = [&](auto &&take) __attribute__((always_inline)) {
+    row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
+      const double t = bins_below(sc, l);
+      if (there && l > -INFINITY && t < (double)kBins && (int)t == bin) {
+        const uint64_t c = composite(l, i);
+        if (c >= from && c <= to) take(c, t);
+      }
+    });
   };
-  auto append = [&](uint64_t *list, bool in, uint64_t c) __attribute__((always_inline)) {
-    const uint64_t mask = __ballot(in);
-    if (mask == 0) return;
-    int at = 0;
-    if (lane == __ffsll((unsigned long long)mask) - 1) at = atomicAdd(&s.n, __popcll(mask));
-    at = __shfl(at, __ffsll((unsigned long long)mask) - 1, 64) + __popcll(mask & ((1ull << lane) - 1));
-    if (in && at < kList) list[at] = c;
-  };
-  auto bounds = [&](uint64_t lo, uint64_t hi) __attribute__((always_inline)) {
+  for (;;) {
+    if (tid == 0) {
+      s.lo = ~0ull;
+      s.hi = 0;
+    }
+    s.sub_mass[tid] = 0;
+    s.sub_count[tid] = 0;
+    __syncthreads();
+    uint64_t lo = ~0ull, hi = 0;
+    each_in([&](uint64_t c, double) __attribute__((always_inline)) {
+      lo = lesser(lo, c);
+      hi = larger(hi, c);
+    });
     hi = wave_max64(hi);
     lo = ~wave_max64(~lo);
     if (lane == 0 && hi) {
       atomicMin((unsigned long long *)&s.lo, (unsigned long long)lo);
       atomicMax((unsigned long long *)&s.hi, (unsigned long long)hi);
     }
-  };
-  {
-    uint64_t lo = ~0ull, hi = 0;
-    row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
-      const bool in = in_bin(l, there);
-      const uint64_t c = in ? composite(l, i) : 0;
-      if (in) {
-        lo = lo < c ? lo : c;
-        hi = hi > c ? hi : c;
-      }
-      append(s.list[0], in, c);
-    });
-    bounds(lo, hi);
-  }
-  __syncthreads();
-  int n = s.n, from_list = 0;
-  bool listed = n <= kList;
-  while (n > 64) {
-    // 1024 further bins over the range that the tokens take; every round leaves at most a 512th of it, and
-    // composites are distinct, so few rounds leave few tokens
-    const uint64_t lo = s.lo, hi = s.hi;
-    const int bits = 64 - __clzll((long long)(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
-    s.sub_mass[tid] = 0;
-    s.sub_count[tid] = 0;
     __syncthreads();
-    if (tid == 0) {
-      s.n = 0;
-      s.lo = ~0ull;
-      s.hi = 0;
-    }
-    auto add = [&](uint64_t c) __attribute__((always_inline)) {
-      const int sub = (int)((hi - c) >> shift);
-      atomicAdd((unsigned long long *)&s.sub_mass[sub], (unsigned long long)weight(sc, s.table, octaves(sc, composite_logit(c))));
+    from = s.lo;
+    to = s.hi;
+    if (from >= to) break;
+    const int bits = 64 - __clzll((long long)(to - from)), shift = bits > 10 ? bits - 10 : 0;
+    each_in([&](uint64_t c, double t) __attribute__((always_inline)) {
+      const int sub = (int)((to - c) >> shift);
+      atomicAdd((unsigned long long *)&s.sub_mass[sub], (unsigned long long)weight(sc, s.table, t));
       atomicAdd(&s.sub_count[sub], 1u);
-    };
-    if (listed) {
-      for (int i = tid; i < n; i += 1024) add(s.list[from_list][i]);
-    } else {
-      row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
-        if (in_bin(l, there)) {
-          const uint64_t c = composite(l, i);
-          if (c >= lo && c <= hi) add(c);
-        }
-      });
+    });
+    __syncthreads();
+    uint64_t m = s.sub_mass[tid];
+    uint32_t c = s.sub_count[tid];
+    const uint64_t own = by_count ? c : m;
+    block_scan(s, m, c);
+    const uint64_t before = by_count ? c : m;
+    if (before <= target && target < before + own) {
+      s.bin[0] = tid;
+      s.upto = m;
+      s.found = before;
     }
     __syncthreads();
-    const uint64_t own_mass = s.sub_mass[tid];
-    const uint32_t own_count = s.sub_count[tid];
+    const uint64_t span = (1ull << shift) - 1;
+    to -= (uint64_t)s.bin[0] << shift;
+    from = to - from > span ? to - span : from;
+    base += s.upto;
+    target -= s.found;
     __syncthreads();
-    prefix<1024>(s.sub_mass, s.sub_count, s);
-    const uint64_t a = by_count ? s.sub_count[tid] : s.sub_mass[tid], more = by_count ? own_count : own_mass;
-    if (a <= target && target < a + more) s.bin = tid;
-    __syncthreads();
-    const int sub = s.bin;
-    const uint64_t new_hi = hi - ((uint64_t)sub << shift), span = ((1ull << shift) - 1);
-    const uint64_t new_lo = new_hi - lo > span ? new_hi - span : lo;
-    target -= by_count ? s.sub_count[sub] : s.sub_mass[sub];
-    base += s.sub_mass[sub];
-    {
-      uint64_t low = ~0ull, high = 0;
-      auto keep = [&](bool in, uint64_t c) __attribute__((always_inline)) {
-        in = in && c >= new_lo && c <= new_hi;
-        if (in) {
-          low = low < c ? low : c;
-          high = high > c ? high : c;
-        }
-        append(s.list[from_list ^ 1], in, c);
-      };
-      if (listed) {
-        for (int i0 = 0; i0 < n; i0 += 1024) {
-          const int i = i0 + tid;
-          keep(i < n, i < n ? s.list[from_list][i] : 0);
-        }
-      } else {
-        row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
-          const bool in = in_bin(l, there);
-          keep(in, in ? composite(l, i) : 0);
-        });
-      }
-      bounds(low, high);
-    }
-    __syncthreads();
-    n = s.n;
-    listed = n <= kList;
-    from_list ^= 1;
   }
-  if (tid < 64) {
-    const uint64_t c = tid < n ? s.list[from_list][tid] : 0;
-    const uint64_t w = tid < n ? weight(sc, s.table, octaves(sc, composite_logit(c))) : 0;
-    uint64_t before = 0;
-    uint32_t rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint64_t cj = __shfl(c, j, 64), wj = __shfl(w, j, 64);
-      if (cj > c) {
-        before += wj;
-        ++rank;
-      }
-    }
-    const bool hit = by_count ? rank == target : before <= target && target < before + w;
-    if (tid < n && hit) {
-      s.found = c;
-      s.upto = base + before + w;
-    }
+  const uint64_t w = weight(sc, s.table, bins_below(sc, composite_logit(from)));
+  __syncthreads();
+  if (tid == 0) {
+    s.found = from;
+    s.upto = base + w;
   }
   __syncthreads();
 }
@@ -441,56 +433,236 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   const int tid = threadIdx.x, r = blockIdx.x;
   const RowSpace &sp = space[r];
   const int64_t was_a = adv.counter_a ? adv.counter_a[0] : 0, was_b = adv.counter_b ? adv.counter_b[0] : 0;
-  const uint64_t best = row_best(sp, slices);
+  // everything that the row's launches left, asked for at once: bins 2 tid and 2 tid + 1
+  const bool has_bins = 2 * tid < kBins;
+  const int at_bins = has_bins ? tid : 0;
+  static_assert(kBins % 2 == 0 && kBins <= 2048, "two bins a thread");
+  const u32x4 masses = reinterpret_cast<const u32x4 *>(sp.mass)[at_bins];
+  const uint64_t two_counts = reinterpret_cast<const uint64_t *>(sp.count)[at_bins];
+  const uint64_t best = row_best(sp, slices), least_sum = sp.least_mass;
   const RowSettings set = row_settings(settings, r);
+  int64_t at = r;
+  if (adv.uniform_index) at = min(max(adv.uniform_index[0], (int64_t)0), (int64_t)adv.n_uniform - 1);
+  const float u = uniform[at];
   int64_t chosen = -1;
   float lp = -INFINITY;
   if (best != 0 && !(set.T > 0.0f)) {
     chosen = composite_index(best);
     lp = 0.0f;
   } else if (best != 0) {
-    const Scale sc = {composite_logit(best), 1.44269504088896340736 / (double)set.T, top};
+    const Scale sc = scale_of(best, set.T, top);
     const Row<dtype> row(logits, stride, r, vocab);
     fill_table(s.table);
     const bool counts = set.top_k > 0;
-    for (int i = tid; i < kBins; i += 1024) {
-      s.mass[i] = sp.mass[i];
-      s.count[i] = counts ? sp.count[i] : 0;
-    }
-    __syncthreads();
-    // the last entry takes the whole: a bin of its own without tokens
     if (tid == 0) {
-      s.mass[kBins] = 0;
-      s.count[kBins] = 0;
+      s.n_pieces = 0;
+      s.n = 0;
+      s.found = best;
+      s.upto = 1ull << top;
+    }
+    // sums and counts in front of the bins: b[0], b[1] of this thread's two, b[2] behind them
+    uint64_t mb[3];
+    uint32_t cb[3];
+    const uint64_t m0 = has_bins ? masses[0] | ((uint64_t)masses[1] << 32) : 0, m1 = has_bins ? masses[2] | ((uint64_t)masses[3] << 32) : 0;
+    const uint32_t c0 = has_bins && counts ? (uint32_t)two_counts : 0, c1 = has_bins && counts ? (uint32_t)(two_counts >> 32) : 0;
+    mb[0] = m0 + m1;
+    cb[0] = c0 + c1;
+    block_scan(s, mb[0], cb[0]);
+    mb[1] = mb[0] + m0, mb[2] = mb[1] + m1;
+    cb[1] = cb[0] + c0, cb[2] = cb[1] + c1;
+    if (2 * tid <= kBins) {              // (the thread behind the bins holds the whole sum)
+      s.mass[2 * tid] = mb[0];
+      s.count[2 * tid] = cb[0];
+      if (has_bins) {
+        s.mass[2 * tid + 1] = mb[1];
+        s.count[2 * tid + 1] = cb[1];
+      }
+    }
+    // the bin where a running sum (count) first exceeds a target that the whole one exceeds
+    auto mark = [&](int slot, uint64_t target) __attribute__((always_inline)) {
+      if (mb[0] <= target && target < mb[2]) s.bin[slot] = 2 * tid + (target >= mb[1] ? 1 : 0);
+    };
+    if (counts && cb[0] < (uint32_t)set.top_k && (uint32_t)set.top_k <= cb[2]) s.bin[0] = 2 * tid + ((uint32_t)set.top_k > cb[1] ? 1 : 0);
+    __syncthreads();
+    const uint64_t total = s.mass[kBins];
+    const bool by_k = counts && (uint32_t)set.top_k < s.count[kBins], by_p = set.top_p < 1.0f;     // (behind the bins the weights are 0)
+    // In which bins the searches can end: top-k's sum is known to within its bin, and so on.  The first token always stays.
+    const uint64_t largest = 1ull << top, least_mass = set.min_p > 0.0f ? larger(least_sum, largest) : ~0ull;
+    uint64_t run_lo = total, run_hi = total;
+    int from[3] = {1, 1, 1}, to[3] = {0, 0, 0};
+    if (by_k) {
+      from[0] = to[0] = s.bin[0];
+      run_lo = larger(s.mass[from[0]], largest);
+      run_hi = s.mass[to[0] + 1];
+    }
+    if (by_p) {
+      mark(1, top_p_target(set.top_p, run_lo));
+      mark(2, top_p_target(set.top_p, run_hi));
+      __syncthreads();
+      from[1] = s.bin[1], to[1] = s.bin[2];
+      run_lo = larger(s.mass[from[1]], largest);
+      run_hi = lesser(run_hi, s.mass[to[1] + 1]);
+    }
+    run_lo = lesser(run_lo, least_mass);
+    run_hi = lesser(run_hi, least_mass);
+    mark(3, token_target(u, run_lo));
+    mark(4, token_target(u, run_hi));
+    __syncthreads();
+    from[2] = s.bin[3], to[2] = s.bin[4];
+    // Pieces of the row that may hold a token of these bins: smallest distances from the three middles.
+    const Near a = near_bins(sc, set.T, by_k ? from[0] : from[2], by_k ? to[0] : to[2]),
+               b = near_bins(sc, set.T, by_p ? from[1] : from[2], by_p ? to[1] : to[2]), c = near_bins(sc, set.T, from[2], to[2]);
+    constexpr int EPP = Row<dtype>::EPP, U = 8;
+    auto scan = [&](auto both) __attribute__((always_inline)) {
+      for (int i0 = 0; i0 < row.pieces; i0 += U * 1024) {
+        u32x4 v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int i = i0 + k * 1024 + tid;
+          v[k] = row.piece(i < row.pieces ? i : 0);
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          float da = INFINITY, db = INFINITY, dc = INFINITY;
+#pragma unroll
+          for (int e = 0; e < EPP; ++e) {
+            const float l = row.value(v[k], e);
+            if (both) {
+              da = fminf(da, fabsf(l - a.middle));
+              db = fminf(db, fabsf(l - b.middle));
+            }
+            dc = fminf(dc, fabsf(l - c.middle));
+          }
+          bool hit = dc <= c.half;
+          if (both) hit |= (da <= a.half) | (db <= b.half);
+          hits |= hit ? 1u << k : 0u;
+        }
+        if (__any(hits != 0)) {
+#pragma unroll 1
+          for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * 1024 + tid;
+            append<uint32_t>(s.pieces, &s.n_pieces, (hits >> k & 1) && i < row.pieces, (uint32_t)i);
+          }
+        }
+      }
+    };
+    struct Yes { __device__ constexpr operator bool() const { return true; } };
+    struct No { __device__ constexpr operator bool() const { return false; } };
+    if (by_k || by_p) scan(Yes{});
+    else scan(No{});
+    __syncthreads();
+    // Their tokens in these bins (and those in front of and behind the pieces).
+    const int n_pieces = s.n_pieces;
+    auto put = [&](float l, int i, bool there) __attribute__((always_inline)) {
+      const double t = bins_below(sc, l);
+      const int bin = (int)t;
+      bool in = false;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) in |= (bin >= from[k]) & (bin <= to[k]);
+      in = in && there && l > -INFINITY && t < (double)kBins;
+      append<uint64_t>(s.list, &s.n, in, in ? composite(l, i) : 0);
+    };
+    if (n_pieces <= kList) {
+      for (int i0 = 0; i0 < n_pieces; i0 += 1024) {
+        const bool there = i0 + tid < n_pieces;
+        const int i = there ? (int)s.pieces[i0 + tid] : 0;
+        const u32x4 v = n_pieces ? row.piece(i) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < EPP; ++e) put(row.value(v, e), row.head + i * EPP + e, there);
+      }
+      const int tail = row.head + row.pieces * EPP, n_ends = row.head + vocab - tail;
+      const int i = tid < row.head ? tid : tail + tid - row.head;
+      put(tid < n_ends ? row.element(i) : 0.0f, i, tid < n_ends);
     }
     __syncthreads();
-    prefix<kBins + 1>(s.mass, s.count, s);
-    uint64_t kept = s.mass[kBins];                                  // of top-k's run
-    if (counts && (uint32_t)set.top_k < s.count[kBins]) {           // (behind the bins the weights are 0)
-      search<dtype>(s, row, sc, true, (uint64_t)(set.top_k - 1));
-      kept = s.upto;
+    const int n = s.n;
+    const bool crowded = n_pieces > kList || n > kList;
+    if (!crowded) {
+      // The list in descending order (bitonic over the next power of two, zeros at the end); then what lies in front of
+      // every token: its bin's, and the bin's tokens in front of it.
+      int size = 64;
+      while (size < n) size *= 2;
+      for (int i = n + tid; i < size; i += 1024) s.list[i] = 0;
+      __syncthreads();
+      for (int k = 2; k <= size; k *= 2) {
+        for (int j = k / 2; j > 0; j /= 2) {
+          for (int q = tid; q < size / 2; q += 1024) {
+            const int x = 2 * q - (q & (j - 1)), y = x + j;
+            const uint64_t lx = s.list[x], ly = s.list[y];
+            if ((lx < ly) == ((x & k) == 0)) {
+              s.list[x] = ly;
+              s.list[y] = lx;
+            }
+          }
+          __syncthreads();
+        }
+      }
+      const int each = size > 1024 ? size / 1024 : 1, first = tid * each, last = min(first + each, n);
+      uint64_t sum = 0;
+#pragma unroll 1
+      for (int i = first; i < last; ++i) {
+        const uint64_t w = weight(sc, s.table, bins_below(sc, composite_logit(s.list[i])));
+        s.own[i] = w;
+        sum += w;
+      }
+      uint32_t unused = 0;
+      block_scan(s, sum, unused);
+#pragma unroll 1
+      for (int i = first; i < last; ++i) {
+        const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
+        if (i == 0 || (int)bins_below(sc, composite_logit(s.list[i - 1])) != bin) {
+          s.run_mass[bin] = sum;
+          s.run_at[bin] = i;
+        }
+        s.before[i] = sum;
+        sum += s.own[i];
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = tid; i < n; i += 1024) {
+        const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
+        s.before[i] += s.mass[bin] - s.run_mass[bin];
+      }
+      __syncthreads();
     }
-    uint64_t run = kept;                                            // of the shortest run
-    if (set.top_p < 1.0f) {
-      const double want = ceil((double)set.top_p * (double)kept);
-      uint64_t target = want >= 1.0 ? (uint64_t)want - 1 : 0;
-      if (target >= kept) target = kept - 1;
-      search<dtype>(s, row, sc, false, target);
-      run = s.upto;
+    uint64_t run = total;                                           // of top-k's run, then of the shortest one
+#pragma unroll 1
+    for (int question = by_k ? 0 : by_p ? 1 : 2; question < 3; ++question) {
+      if (question == 1 && !by_p) continue;
+      if (question == 2) run = lesser(run, least_mass);
+      const bool by_count = question == 0;
+      const uint64_t target = by_count ? (uint64_t)(set.top_k - 1) : question == 1 ? top_p_target(set.top_p, run) : token_target(u, run);
+      if (!crowded) {
+#pragma unroll 1
+        for (int i = tid; i < n; i += 1024) {
+          const uint64_t before = s.before[i], w = s.own[i];
+          bool hit = before <= target && target < before + w;
+          if (by_count) {
+            const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
+            hit = bin == from[0] && (uint64_t)(s.count[bin] + (i - s.run_at[bin])) == target;
+          }
+          if (hit) {
+            s.found = s.list[i];
+            s.upto = before + w;
+          }
+        }
+      } else {
+        const uint64_t t0 = by_count ? cb[0] : mb[0], t1 = by_count ? cb[1] : mb[1], t2 = by_count ? cb[2] : mb[2];
+        if (t0 <= target && target < t2) s.bin[0] = 2 * tid + (target >= t1 ? 1 : 0);
+        __syncthreads();
+        const int bin = s.bin[0];
+        __syncthreads();
+        crowded_search<dtype>(s, row, sc, bin, by_count, target - (by_count ? s.count[bin] : s.mass[bin]));
+      }
+      __syncthreads();
+      if (question < 2) {
+        run = s.upto;
+        __syncthreads();
+      }
     }
-    if (set.min_p > 0.0f) {
-      const uint64_t largest = 1ull << top;                         // the first token always stays
-      const uint64_t least = sp.least_mass > largest ? sp.least_mass : largest;
-      run = run < least ? run : least;
-    }
-    int64_t at = r;
-    if (adv.uniform_index) at = min(max(adv.uniform_index[0], (int64_t)0), (int64_t)adv.n_uniform - 1);
-    const double x = (double)uniform[at] * (double)run;
-    uint64_t target = x > 0.0 ? (x < (double)run ? (uint64_t)x : run - 1) : 0;
-    if (target >= run) target = run - 1;
-    search<dtype>(s, row, sc, false, target);
     chosen = composite_index(s.found);
-    lp = (float)(-octaves(sc, composite_logit(s.found)) * 0.693147180559945309417 - log(ldexp((double)run, -top)));
+    lp = (float)(-bins_below(sc, composite_logit(s.found)) * (0.693147180559945309417 / kPerOctave) - log(ldexp((double)run, -top)));
   }
   if (tid == 0) {
     token[r] = chosen;
