@@ -414,8 +414,8 @@ int rdkv_w4_linear_silu(const void *codes, const uint32_t *scales, const void *g
  *   top_p of theirs; min_p > 0: tokens with w_i >= min_p; the first token always stays;
  *   token = the first one whose running sum exceeds uniform * the sum of those that stay (uniform in [0, 1)),
  *   logprob = the log of its share of that sum.
- * A temperature that is not above 0 takes the largest logit (logprob 0).  NaN and -inf are masked; a logit of +inf
- * leaves the others without weight; a row with nothing left has token -1 and logprob -inf.  Weights and sums are
+ * A temperature that is not above 0 takes the largest logit (logprob 0).  NaN and -inf are masked, +inf counts as
+ * the largest number of fp32; a row with nothing left has token -1 and logprob -inf.  Weights and sums are
  * held in 64 bits: the same token whatever the batch.  A member of RdkvSampling that is not NULL holds one value per
  * row (device memory), else its _value counts. */
 typedef struct RdkvSampling {

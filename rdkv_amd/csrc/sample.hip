@@ -10,7 +10,7 @@
 // so that a sum does not depend on the order, the launch's shape or the atomics that form it, and a border between two
 // tokens lies where 64 bits put it.
 //
-// Three launches.  Maximum: the slices of a row leave their largest logit and its place.  Histogram: sums (and, under top-k,
+// Three launches.  Maximum: the slices of a row leave their largest logit.  Histogram: sums (and, under top-k,
 // counts) of the weights in bins of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup
 // per row adds the bins up, which tells in which bins the searches can end, collects those bins' tokens in one pass over the
 // row and resolves the searches among them, by further bins over (logit, index) while they are many.
@@ -27,7 +27,7 @@ constexpr int kMaxVocab = 1 << 24;
 
 // Workspace of a row: the slices' maxima, then the histogram.
 struct RowSpace {
-  uint64_t best[kMaxSlices];             // ordered logit << 32 | ~index, 0: nothing allowed
+  float best[kMaxSlices];                // -inf: nothing allowed
   uint64_t least_mass;                   // sum of the weights of at least min_p
   uint64_t pad;
   uint64_t mass[kBins];
@@ -52,9 +52,8 @@ __device__ __forceinline__ RowSettings row_settings(const Settings &s, int row) 
   return r;
 }
 
-// A logit and its index as one number in the tokens' order (larger first); 0 where the token is masked (-inf, NaN).
+// A logit and its index as one number in the tokens' order (larger first).
 __device__ __forceinline__ uint64_t composite(float l, int index) {
-  if (!(l > -INFINITY)) return 0;
   return ((uint64_t)rdkv_float_to_ordered(l + 0.0f) << 32) | (uint32_t)~index;     // (-0 counts as 0)
 }
 __device__ __forceinline__ float composite_logit(uint64_t c) { return rdkv_ordered_to_float((uint32_t)(c >> 32)); }
@@ -62,14 +61,17 @@ __device__ __forceinline__ int composite_index(uint64_t c) { return (int)~(uint3
 
 // Bins below the maximum, in fp64 (the bin, and the place in it), and the weight there.  Two launches form them and add
 // them up to the same sums, bit for bit: nothing is contracted that is not written as fma.
-struct Scale { float m; double inv; int top; };     // maximum, bins per unit of logit, weight 2^top of the maximum
-__device__ __forceinline__ Scale scale_of(uint64_t best, float T, int top) {
-  return Scale{rdkv_ordered_to_float((uint32_t)(best >> 32)), 1.44269504088896340736 * kPerOctave / (double)T, top};
+// A logit of +inf counts as the largest number of fp32.
+struct Scale { double m, inv; int top; };           // maximum, bins per unit of logit, weight 2^top of the maximum
+__device__ __forceinline__ Scale scale_of(float best, float T, int top) {
+  return Scale{(double)fminf(best, 3.402823466e38f), fmax(1.44269504088896340736 * kPerOctave / (double)T, 1e-300), top};
 }
+// NaN for NaN, infinite for -inf, negative for +inf: the caller's comparison and `placed` put these right.
 __device__ __forceinline__ double bins_below(const Scale &s, float l) {
 #pragma clang fp contract(off)
-  return l == s.m ? 0.0 : ((double)s.m - (double)l) * s.inv;
+  return (s.m - (double)l) * s.inv;
 }
+__device__ __forceinline__ double placed(double t) { return fmax(t, 0.0); }
 // 2^(top - t / 32) as an integer: 2^(52 - i / 32) of the bin's place in its octave from the table, times the series of
 // 2^(-f / 32) for the rest f < 1 (2e-13 of it left out), added to 2^52 for its bits as an integer, shifted.
 __device__ __forceinline__ uint64_t weight(const Scale &s, const double *table, double t) {
@@ -155,7 +157,7 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 template <int dtype>
 __global__ void __launch_bounds__(256)
 sample_max_kernel(const void *__restrict__ logits, int64_t stride, int vocab, RowSpace *__restrict__ space) {
-  __shared__ uint64_t s_best[4];
+  __shared__ float s_best[4];
   const int slice = blockIdx.x, slices = gridDim.x, tid = threadIdx.x;
   RowSpace &sp = space[blockIdx.y];
   for (int i = slice * 256 + tid; i < kBins; i += slices * 256) {
@@ -165,23 +167,19 @@ sample_max_kernel(const void *__restrict__ logits, int64_t stride, int vocab, Ro
   if (slice == 0 && tid == 0) sp.least_mass = 0;
   const Row<dtype> row(logits, stride, blockIdx.y, vocab);
   const int per = (row.pieces + slices - 1) / slices, begin = min(slice * per, row.pieces), end = min(begin + per, row.pieces);
-  uint64_t best = 0;
-  row.template each<256>(begin, end, slice == 0, [&](float l, int i, bool there) __attribute__((always_inline)) {
-    const uint64_t c = there ? composite(l, i) : 0;
-    best = best > c ? best : c;
+  float best = -INFINITY;                // (a NaN is never the larger one)
+  row.template each<256>(begin, end, slice == 0, [&](float l, int, bool there) __attribute__((always_inline)) {
+    best = fmaxf(best, there ? l : -INFINITY);
   });
-  best = wave_max64(best);
+  best = rdkv_wave_max(best);
   if ((tid & 63) == 0) s_best[tid >> 6] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 4; ++w) best = best > s_best[w] ? best : s_best[w];
-    sp.best[slice] = best;
-  }
+  if (tid == 0) sp.best[slice] = fmaxf(fmaxf(s_best[0], s_best[1]), fmaxf(s_best[2], s_best[3]));
 }
 
-__device__ __forceinline__ uint64_t row_best(const RowSpace &sp, int slices) {
+__device__ __forceinline__ float row_best(const RowSpace &sp, int slices) {
   const int lane = threadIdx.x & 63;
-  return wave_max64(lane < slices ? sp.best[lane] : 0);
+  return rdkv_wave_max(lane < slices ? sp.best[lane] : -INFINITY);
 }
 
 template <int dtype>
@@ -194,9 +192,9 @@ sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, i
   __shared__ uint64_t s_least;
   const int slice = blockIdx.x, slices = gridDim.x, tid = threadIdx.x;
   RowSpace &sp = space[blockIdx.y];
-  const uint64_t best = row_best(sp, slices);
+  const float best = row_best(sp, slices);
   const RowSettings set = row_settings(settings, blockIdx.y);
-  if (best == 0 || !(set.T > 0.0f)) return;              // nothing allowed, or the largest is the choice
+  if (best == -INFINITY || !(set.T > 0.0f)) return;      // nothing allowed, or the largest is the choice
   const bool counts = set.top_k > 0, least = set.min_p > 0.0f;
   fill_table(s_table);
   for (int i = tid; i < kBins; i += 256) {
@@ -213,8 +211,9 @@ sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, i
   const int per = (row.pieces + slices - 1) / slices, begin = min(slice * per, row.pieces), end = min(begin + per, row.pieces);
   uint64_t least_mass = 0;
   row.template each<256>(begin, end, slice == 0, [&](float l, int i, bool there) __attribute__((always_inline)) {
-    const double t = bins_below(sc, l);
-    if (there && l > -INFINITY && t < need) {
+    double t = bins_below(sc, l);
+    if (t < (there ? need : -INFINITY)) {
+      t = placed(t);
       const uint64_t w = weight(sc, s_table, t);
       const int bin = (int)t;
       atomicAdd((unsigned long long *)&s_mass[bin], (unsigned long long)w);
@@ -246,10 +245,13 @@ constexpr int kList = 4096;              // tokens that the last launch sorts, a
 struct Choice {                          // LDS of the last launch
   uint64_t mass[kBins + 1];              // sums (counts) in front of a bin, the whole at the end
   uint32_t count[kBins + 1];
-  uint64_t list[kList];                  // the tokens of the searches' bins; sorted, with the sum in front of each and
-  uint64_t before[kList], own[kList];    // its own weight
+  uint64_t list[kList];                  // the tokens of the searches' bins, sorted
   union {
-    uint32_t pieces[kList];              // pieces of the row that may hold one
+    u32x4 piece[kList];                  // pieces of the row that may hold one
+    struct { uint64_t before[kList], own[kList]; };      // the sum in front of each token of the list, its weight
+  };
+  union {
+    uint32_t pieces[kList];              // the pieces' numbers
     struct {                             // of the sorted list, where a bin's run starts: its sum and its place
       uint64_t run_mass[kBins];
       uint32_t run_at[kBins];
@@ -312,16 +314,15 @@ __device__ __forceinline__ void block_scan(Choice &s, uint64_t &m, uint32_t &c) 
   c = bc;
 }
 
-// Puts v into the list of every lane whose `in` holds (the whole wavefront takes part); *n counts them all.
-template <class T>
-__device__ __forceinline__ void append(T *list, int *n, bool in, T v) {
+// A place in a list for every lane whose `in` holds (the whole wavefront takes part); *n counts them all.
+__device__ __forceinline__ int place_in(int *n, bool in) {
   const uint64_t mask = __ballot(in);
-  if (mask == 0) return;
+  if (mask == 0) return kList;
   const int lane = threadIdx.x & 63, first = __ffsll((unsigned long long)mask) - 1;
   int at = 0;
   if (lane == first) at = atomicAdd(n, __popcll(mask));
   at = __shfl(at, first, 64) + __popcll(mask & ((1ull << lane) - 1));
-  if (in && at < kList) list[at] = v;
+  return in ? at : kList;
 }
 
 // Logits that can lie in bins [from, to] as a distance from a middle, wide enough for every rounding on the way; what is
@@ -329,10 +330,11 @@ __device__ __forceinline__ void append(T *list, int *n, bool in, T v) {
 struct Near { float middle, half; };
 __device__ __forceinline__ Near near_bins(const Scale &sc, float T, int from, int to) {
   const double w = (double)T * (0.693147180559945309417 / kPerOctave);      // logits a bin
-  const double lo = (double)sc.m - ((double)to + 1.001) * w, hi = (double)sc.m - ((double)from - 0.001) * w;
+  const double lo = sc.m - ((double)to + 1.001) * w, hi = sc.m - ((double)from - 0.001) * w;
   Near n = {(float)(0.5 * (lo + hi)), (float)(0.5 * (hi - lo))};
   n.half += n.half * 0x1p-20f + fabsf(n.middle) * 0x1p-22f;
-  if (!(fabsf(n.middle) < INFINITY) || !(n.half < INFINITY)) n = Near{0.0f, INFINITY};
+  // (+inf counts as the largest number: where that can be in reach, every piece is looked into)
+  if (!(fabsf(n.middle) < 1e38f) || !(n.half < 1e38f)) n = Near{0.0f, INFINITY};
   return n;
 }
 
@@ -360,9 +362,9 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
   auto each_in = [&](auto &&take) __attribute__((always_inline)) {
     row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
       const double t = bins_below(sc, l);
-      if (there && l > -INFINITY && t < (double)kBins && (int)t == bin) {
+      if (there && t < (double)kBins && (int)placed(t) == bin) {
         const uint64_t c = composite(l, i);
-        if (c >= from && c <= to) take(c, t);
+        if (c >= from && c <= to) take(c, placed(t));
       }
     });
   };
@@ -414,7 +416,7 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
     target -= s.found;
     __syncthreads();
   }
-  const uint64_t w = weight(sc, s.table, bins_below(sc, composite_logit(from)));
+  const uint64_t w = weight(sc, s.table, placed(bins_below(sc, composite_logit(from))));
   __syncthreads();
   if (tid == 0) {
     s.found = from;
@@ -439,26 +441,35 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   static_assert(kBins % 2 == 0 && kBins <= 2048, "two bins a thread");
   const u32x4 masses = reinterpret_cast<const u32x4 *>(sp.mass)[at_bins];
   const uint64_t two_counts = reinterpret_cast<const uint64_t *>(sp.count)[at_bins];
-  const uint64_t best = row_best(sp, slices), least_sum = sp.least_mass;
+  const uint64_t least_sum = sp.least_mass;
+  const float best = row_best(sp, slices);
   const RowSettings set = row_settings(settings, r);
   int64_t at = r;
   if (adv.uniform_index) at = min(max(adv.uniform_index[0], (int64_t)0), (int64_t)adv.n_uniform - 1);
   const float u = uniform[at];
   int64_t chosen = -1;
   float lp = -INFINITY;
-  if (best != 0 && !(set.T > 0.0f)) {
-    chosen = composite_index(best);
+  const Row<dtype> row(logits, stride, r, vocab);
+  if (best > -INFINITY && !(set.T > 0.0f)) {             // the first place of the largest
+    if (tid == 0) s.n = 0x7fffffff;
+    __syncthreads();
+    int first = 0x7fffffff;
+    row.template each<1024>(0, row.pieces, true, [&](float l, int i, bool there) __attribute__((always_inline)) {
+      first = there && l == best ? min(first, i) : first;
+    });
+    if (first != 0x7fffffff) atomicMin(&s.n, first);
+    __syncthreads();
+    chosen = s.n;
     lp = 0.0f;
-  } else if (best != 0) {
+  } else if (best > -INFINITY) {
     const Scale sc = scale_of(best, set.T, top);
-    const Row<dtype> row(logits, stride, r, vocab);
     fill_table(s.table);
     const bool counts = set.top_k > 0;
     if (tid == 0) {
       s.n_pieces = 0;
       s.n = 0;
-      s.found = best;
-      s.upto = 1ull << top;
+      s.found = ~0ull;                   // (index 0)
+      s.upto = 0;
     }
     // sums and counts in front of the bins: b[0], b[1] of this thread's two, b[2] behind them
     uint64_t mb[3];
@@ -539,10 +550,13 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
           hits |= hit ? 1u << k : 0u;
         }
         if (__any(hits != 0)) {
-#pragma unroll 1
+#pragma unroll
           for (int k = 0; k < U; ++k) {
-            const int i = i0 + k * 1024 + tid;
-            append<uint32_t>(s.pieces, &s.n_pieces, (hits >> k & 1) && i < row.pieces, (uint32_t)i);
+            const int i = i0 + k * 1024 + tid, at = place_in(&s.n_pieces, (hits >> k & 1) && i < row.pieces);
+            if (at < kList) {
+              s.pieces[at] = (uint32_t)i;
+              s.piece[at] = v[k];
+            }
           }
         }
       }
@@ -556,18 +570,18 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
     const int n_pieces = s.n_pieces;
     auto put = [&](float l, int i, bool there) __attribute__((always_inline)) {
       const double t = bins_below(sc, l);
-      const int bin = (int)t;
+      const int bin = (int)placed(t);
       bool in = false;
 #pragma unroll
       for (int k = 0; k < 3; ++k) in |= (bin >= from[k]) & (bin <= to[k]);
-      in = in && there && l > -INFINITY && t < (double)kBins;
-      append<uint64_t>(s.list, &s.n, in, in ? composite(l, i) : 0);
+      const int at = place_in(&s.n, in && there && t < (double)kBins);
+      if (at < kList) s.list[at] = composite(l, i);
     };
     if (n_pieces <= kList) {
       for (int i0 = 0; i0 < n_pieces; i0 += 1024) {
         const bool there = i0 + tid < n_pieces;
-        const int i = there ? (int)s.pieces[i0 + tid] : 0;
-        const u32x4 v = n_pieces ? row.piece(i) : u32x4{0, 0, 0, 0};
+        const int q = there ? i0 + tid : 0, i = (int)s.pieces[q];
+        const u32x4 v = s.piece[q];
 #pragma unroll
         for (int e = 0; e < EPP; ++e) put(row.value(v, e), row.head + i * EPP + e, there);
       }
@@ -580,29 +594,52 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
     const bool crowded = n_pieces > kList || n > kList;
     if (!crowded) {
       // The list in descending order (bitonic over the next power of two, zeros at the end); then what lies in front of
-      // every token: its bin's, and the bin's tokens in front of it.
+      // every token: its bin's, and the bin's tokens in front of it.  Up to 1024 tokens: one a thread, partners within a
+      // wavefront through registers, LDS and barriers only for the further ones.
       int size = 64;
       while (size < n) size *= 2;
-      for (int i = n + tid; i < size; i += 1024) s.list[i] = 0;
-      __syncthreads();
-      for (int k = 2; k <= size; k *= 2) {
-        for (int j = k / 2; j > 0; j /= 2) {
-          for (int q = tid; q < size / 2; q += 1024) {
-            const int x = 2 * q - (q & (j - 1)), y = x + j;
-            const uint64_t lx = s.list[x], ly = s.list[y];
-            if ((lx < ly) == ((x & k) == 0)) {
-              s.list[x] = ly;
-              s.list[y] = lx;
-            }
+      if (size <= 1024) {
+        uint64_t v = tid < n ? s.list[tid] : 0;
+        for (int k = 2; k <= size; k *= 2) {
+          const bool down = (tid & k) == 0;
+          for (int j = k / 2; j >= 64; j /= 2) {
+            __syncthreads();
+            if (tid < size) s.list[tid] = v;
+            __syncthreads();
+            const uint64_t other = tid < size ? s.list[tid ^ j] : 0;
+            v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
           }
-          __syncthreads();
+          for (int j = k / 2 < 32 ? k / 2 : 32; j > 0; j /= 2) {
+            const uint64_t other = __shfl_xor(v, j, 64);
+            v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
+          }
+        }
+        __syncthreads();
+        if (tid < n) s.list[tid] = v;
+        __syncthreads();
+      } else {
+        for (int i = n + tid; i < size; i += 1024) s.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= size; k *= 2) {
+          for (int j = k / 2; j > 0; j /= 2) {
+            for (int q = tid; q < size / 2; q += 1024) {
+              const int x = 2 * q - (q & (j - 1)), y = x + j;
+              const uint64_t lx = s.list[x], ly = s.list[y];
+              if ((lx < ly) == ((x & k) == 0)) {
+                s.list[x] = ly;
+                s.list[y] = lx;
+              }
+            }
+            __syncthreads();
+          }
         }
       }
+      auto bin_at = [&](int i) __attribute__((always_inline)) { return (int)placed(bins_below(sc, composite_logit(s.list[i]))); };
       const int each = size > 1024 ? size / 1024 : 1, first = tid * each, last = min(first + each, n);
       uint64_t sum = 0;
 #pragma unroll 1
       for (int i = first; i < last; ++i) {
-        const uint64_t w = weight(sc, s.table, bins_below(sc, composite_logit(s.list[i])));
+        const uint64_t w = weight(sc, s.table, placed(bins_below(sc, composite_logit(s.list[i]))));
         s.own[i] = w;
         sum += w;
       }
@@ -610,8 +647,8 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       block_scan(s, sum, unused);
 #pragma unroll 1
       for (int i = first; i < last; ++i) {
-        const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
-        if (i == 0 || (int)bins_below(sc, composite_logit(s.list[i - 1])) != bin) {
+        const int bin = bin_at(i);
+        if (i == 0 || bin_at(i - 1) != bin) {
           s.run_mass[bin] = sum;
           s.run_at[bin] = i;
         }
@@ -621,7 +658,7 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       __syncthreads();
 #pragma unroll 1
       for (int i = tid; i < n; i += 1024) {
-        const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
+        const int bin = bin_at(i);
         s.before[i] += s.mass[bin] - s.run_mass[bin];
       }
       __syncthreads();
@@ -639,7 +676,7 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
           const uint64_t before = s.before[i], w = s.own[i];
           bool hit = before <= target && target < before + w;
           if (by_count) {
-            const int bin = (int)bins_below(sc, composite_logit(s.list[i]));
+            const int bin = (int)placed(bins_below(sc, composite_logit(s.list[i])));
             hit = bin == from[0] && (uint64_t)(s.count[bin] + (i - s.run_at[bin])) == target;
           }
           if (hit) {
@@ -662,7 +699,7 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       }
     }
     chosen = composite_index(s.found);
-    lp = (float)(-bins_below(sc, composite_logit(s.found)) * (0.693147180559945309417 / kPerOctave) - log(ldexp((double)run, -top)));
+    lp = (float)(-placed(bins_below(sc, composite_logit(s.found))) * (0.693147180559945309417 / kPerOctave) - log(ldexp((double)run, -top)));
   }
   if (tid == 0) {
     token[r] = chosen;
