@@ -245,7 +245,8 @@ constexpr int kList = 4096;              // tokens that the last launch sorts, a
 struct Choice {                          // LDS of the last launch
   uint64_t mass[kBins + 1];              // sums (counts) in front of a bin, the whole at the end
   uint32_t count[kBins + 1];
-  uint64_t list[kList];                  // the tokens of the searches' bins, sorted
+  uint64_t list[kList];                  // the tokens of the searches' bins
+  uint32_t rank[kList];                  // and how many are in front of each
   union {
     u32x4 piece[kList];                  // pieces of the row that may hold one
     struct { uint64_t before[kList], own[kList]; };      // the sum in front of each token of the list, its weight
@@ -292,6 +293,33 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   v += moved<0x118, 0xf>(v);
   v += moved<0x142, 0xa>(v);
   return v + moved<0x143, 0xc>(v);
+}
+// The sum over a wavefront, in its last lane (fewer moves than the sums in front of every lane).
+template <class T, int CTRL>
+__device__ __forceinline__ T partner(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, CTRL, 0xf, 0xf, true),
+                   hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, true);
+    return ((uint64_t)hi << 32) | lo;
+  } else {
+    return (T)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+  }
+}
+__device__ __forceinline__ uint64_t handed_on(uint64_t v) {
+  v += moved64<0x142, 0xa>(v);
+  return v + moved64<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint32_t handed_on(uint32_t v) {
+  v += moved<0x142, 0xa>(v);
+  return v + moved<0x143, 0xc>(v);
+}
+template <class T>
+__device__ __forceinline__ T wave_total(T v) {
+  v += partner<T, 0xb1>(v);              // pairs, fours, eights, sixteens
+  v += partner<T, 0x4e>(v);
+  v += partner<T, 0x141>(v);
+  v += partner<T, 0x140>(v);
+  return handed_on(v);
 }
 // Sums over the workgroup's threads in front of this one.
 __device__ __forceinline__ void block_scan(Choice &s, uint64_t &m, uint32_t &c) {
@@ -547,16 +575,20 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
           }
           bool hit = dc <= c.half;
           if (both) hit |= (da <= a.half) | (db <= b.half);
-          hits |= hit ? 1u << k : 0u;
+          hits |= hit && i0 + k * 1024 + tid < row.pieces ? 1u << k : 0u;
         }
-        if (__any(hits != 0)) {
+        if (__any(hits != 0)) {          // places in the list for all of the wavefront's pieces at once
+          const uint32_t own = __popc(hits), upto = wave_scan(own);
+          int at = 0;
+          if ((tid & 63) == 63) at = atomicAdd(&s.n_pieces, (int)upto);
+          at = __builtin_amdgcn_readlane(at, 63) + (int)(upto - own);
 #pragma unroll
           for (int k = 0; k < U; ++k) {
-            const int i = i0 + k * 1024 + tid, at = place_in(&s.n_pieces, (hits >> k & 1) && i < row.pieces);
-            if (at < kList) {
-              s.pieces[at] = (uint32_t)i;
+            if ((hits >> k & 1) && at < kList) {
+              s.pieces[at] = (uint32_t)(i0 + k * 1024 + tid);
               s.piece[at] = v[k];
             }
+            at += hits >> k & 1;
           }
         }
       }
@@ -592,11 +624,35 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
     __syncthreads();
     const int n = s.n;
     const bool crowded = n_pieces > kList || n > kList;
-    if (!crowded) {
+    if (n <= 64 && !crowded) {
+      // a lane each: a token's bin's sum and count, and those of the bin's tokens in front of it
+      if (tid < 64) {
+        const uint64_t c = tid < n ? s.list[tid] : 0;
+        const double t = placed(bins_below(sc, composite_logit(c)));
+        const int bin = tid < n ? (int)t : 0;
+        const uint64_t w = weight(sc, s.table, tid < n ? t : 0.0);
+        uint64_t before = s.mass[bin];
+        uint32_t rank = s.count[bin];
+        for (int j = 0; j < n; ++j) {
+          auto of = [&](uint64_t x) __attribute__((always_inline)) {
+            return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), j) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, j);
+          };
+          const bool front = of(c) > c && __builtin_amdgcn_readlane(bin, j) == bin;
+          before += front ? of(w) : 0;
+          rank += front ? 1 : 0;
+        }
+        if (tid < n) {
+          s.before[tid] = before;
+          s.own[tid] = w;
+          s.rank[tid] = rank;
+        }
+      }
+      __syncthreads();
+    } else if (!crowded) {
       // The list in descending order (bitonic over the next power of two, zeros at the end); then what lies in front of
       // every token: its bin's, and the bin's tokens in front of it.  Up to 1024 tokens: one a thread, partners within a
       // wavefront through registers, LDS and barriers only for the further ones.
-      int size = 64;
+      int size = 128;
       while (size < n) size *= 2;
       if (size <= 1024) {
         uint64_t v = tid < n ? s.list[tid] : 0;
@@ -609,9 +665,16 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
             const uint64_t other = tid < size ? s.list[tid ^ j] : 0;
             v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
           }
-          for (int j = k / 2 < 32 ? k / 2 : 32; j > 0; j /= 2) {
-            const uint64_t other = __shfl_xor(v, j, 64);
+          auto with = [&](int j, uint64_t other) __attribute__((always_inline)) {
             v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
+          };
+          if (tid < size) {              // (whole wavefronts)
+            if (k >= 64) with(32, __shfl_xor(v, 32, 64));
+            if (k >= 32) with(16, __shfl_xor(v, 16, 64));
+            if (k >= 16) with(8, partner<uint64_t, 0x128>(v));
+            if (k >= 8) with(4, partner<uint64_t, 0x1b>(partner<uint64_t, 0x141>(v)));      // 7 ^ 3
+            if (k >= 4) with(2, partner<uint64_t, 0x4e>(v));
+            with(1, partner<uint64_t, 0xb1>(v));
           }
         }
         __syncthreads();
@@ -660,6 +723,7 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       for (int i = tid; i < n; i += 1024) {
         const int bin = bin_at(i);
         s.before[i] += s.mass[bin] - s.run_mass[bin];
+        s.rank[i] = s.count[bin] + (i - s.run_at[bin]);
       }
       __syncthreads();
     }
@@ -674,11 +738,7 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
 #pragma unroll 1
         for (int i = tid; i < n; i += 1024) {
           const uint64_t before = s.before[i], w = s.own[i];
-          bool hit = before <= target && target < before + w;
-          if (by_count) {
-            const int bin = (int)placed(bins_below(sc, composite_logit(s.list[i])));
-            hit = bin == from[0] && (uint64_t)(s.count[bin] + (i - s.run_at[bin])) == target;
-          }
+          const bool hit = by_count ? s.rank[i] == (uint32_t)target : before <= target && target < before + w;
           if (hit) {
             s.found = s.list[i];
             s.upto = before + w;
@@ -713,6 +773,392 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   if (tid < adv.n_counts) adv.counts[tid] += 1;
 }
 
+// ---- 16-bit logits ----------------------------------------------------------------------------------
+// A row of 16-bit logits holds few different values, so one pass that counts them is all that most of the work needs: the
+// weight of a value is formed once, sums over values are counts times weights, and the questions are asked of values.
+// One workgroup per row, one launch: LDS holds a 16-bit counter for every one of the 2^16 bit patterns (two to a word), in
+// the values' order; a thread owns four blocks of 16 neighbouring patterns and forms their sums (smaller blocks share the
+// crowded values out over more wavefronts, and cost more sums over the workgroup).  Only the
+// token itself needs the row again: the place of its value's n-th occurrence.  A pattern that occurs 2^16 times or more
+// shows in the counters' sum; the patterns are then counted again with 32 bits, half of them at a time.
+struct Values {                          // LDS
+  uint32_t words[1 << 15];               // counter of key k: word_of(k), its half k / 2^15 (or all of it, of one half)
+  uint64_t part_mass[4][16];
+  uint32_t part_count[4][16];
+  double table[kPerOctave];
+  uint64_t least, base_mass, upto;
+  uint32_t total, base_count, place, seg_count[18];
+  int max_key, group, key, seg_first[18], index;
+};
+// Neighbouring keys lie in neighbouring banks, and so do keys 32 apart (a thread reads 16 neighbours).
+__device__ __forceinline__ uint32_t word_of(uint32_t key) { return (key & 0x7fffu) ^ ((key >> 5) & 31u); }
+
+template <int dtype>
+__global__ void __launch_bounds__(1024)
+sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, Settings settings,
+                     const float *__restrict__ uniform, int64_t *__restrict__ token, float *__restrict__ logprob, Advance adv) {
+  extern __shared__ char lds[];
+  Values &s = *reinterpret_cast<Values *>(lds);
+  constexpr int kInf = dtype == RDKV_DTYPE_F16 ? 0x7c00 : 0x7f80, U = 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = blockIdx.x;
+  const int64_t was_a = adv.counter_a ? adv.counter_a[0] : 0, was_b = adv.counter_b ? adv.counter_b[0] : 0;
+  const RowSettings set = row_settings(settings, r);
+  int64_t at = r;
+  if (adv.uniform_index) at = min(max(adv.uniform_index[0], (int64_t)0), (int64_t)adv.n_uniform - 1);
+  const float u = uniform[at];
+  const Row<dtype> row(logits, stride, r, vocab);
+  // keys: the bit patterns in the order of their values; NaN's lie beyond the infinities'
+  auto allowed = [](int key) __attribute__((always_inline)) { return key > 0x7fff - kInf && key <= 0x8000 + kInf; };
+  auto value = [](int key) __attribute__((always_inline)) {
+    const uint16_t bits = (uint16_t)(key & 0x8000 ? key & 0x7fff : ~key);
+    return dtype == RDKV_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, bits) : __uint_as_float((uint32_t)bits << 16);
+  };
+  // Counts the row: both halves of the keys in 16 bits each, or (half 0 or 1) those of one half in 32.
+  auto count = [&](int half) __attribute__((always_inline)) {
+    u32x4 *words = reinterpret_cast<u32x4 *>(s.words);
+#pragma unroll
+    for (int i = 0; i < (1 << 13) / 1024; ++i) words[i * 1024 + tid] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    auto one = [&](uint32_t key) __attribute__((always_inline)) {        // (the upper half is not looked at)
+      const uint32_t upper = (key >> 15) & 1;
+      if (half < 0) atomicAdd(&s.words[word_of(key)], upper * 0xffffu + 1u);
+      else if ((int)upper == half) atomicAdd(&s.words[word_of(key)], 1u);
+    };
+    auto two = [&](uint32_t bits) __attribute__((always_inline)) {
+      if (half >= 0) {                                                  // (-0 counts as 0)
+        if ((bits & 0xffffu) == 0x8000u) bits &= 0xffff0000u;
+        if ((bits >> 16) == 0x8000u) bits &= 0xffffu;
+      }
+      typedef short short2_t __attribute__((ext_vector_type(2)));
+      const uint32_t negative = __builtin_bit_cast(uint32_t, __builtin_bit_cast(short2_t, bits) >> (short)15);
+      const uint32_t keys = bits ^ (negative | 0x80008000u);
+      one(keys);
+      one(keys >> 16);
+    };
+    for (int i0 = 0; i0 < row.pieces; i0 += U * 1024) {
+      u32x4 v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * 1024 + tid;
+        v[k] = row.piece(i < row.pieces ? i : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i0 + k * 1024 + tid < row.pieces) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t pair = v[k][e];
+            two(pair);
+          }
+        }
+      }
+    }
+    const int tail = row.head + row.pieces * 8, n_ends = row.head + vocab - tail;
+    if (tid < n_ends) {
+      uint32_t bits = reinterpret_cast<const uint16_t *>(row.p)[tid < row.head ? tid : tail + tid - row.head];
+      if (half >= 0 && bits == 0x8000u) bits = 0;
+      one(bits ^ (0x8000u | ((bits >> 15) * 0x7fffu)));
+    }
+    __syncthreads();
+  };
+  int half = -1;
+  auto counter = [&](int key) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t w = s.words[word_of(key)];
+    return half < 0 ? (key & 0x8000 ? w >> 16 : w & 0xffffu) : (key >> 15) == half ? w : 0;
+  };
+  fill_table(s.table);
+  if (tid == 0) {
+    s.least = 0;
+    s.total = 0;
+    s.max_key = -1;
+  }
+  count(-1);
+  if (tid == 0) {          // -0 joins 0, its neighbour
+    uint32_t &minus = s.words[word_of(0x7fff)], &zero = s.words[word_of(0x8000)];
+    const uint32_t c = minus & 0xffffu;
+    if (c + (zero >> 16) <= 0xffffu) {
+      zero += c << 16;
+      minus -= c;
+    } else {
+      s.total = 1;         // (the sum will not be the row's length)
+    }
+  }
+  __syncthreads();
+  // Which of the thread's keys occur, the largest of all, and, for the 16-bit counters, the sum of all.  Block b of the thread:
+  // keys 16 (tid + 1024 b) and on; the blocks b and b + 2 share their words.
+  uint32_t occur[2] = {0, 0};            // blocks b (lower 16 bits) and b + 2
+  static_assert(kInf % 16 == 0, "a block's keys are on one side of an infinity, but for itself");
+  int max_key = -1;
+  auto look = [&]() __attribute__((always_inline)) {
+    uint32_t total = 0;
+    int largest = -1;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int first = 16 * tid + 16384 * b;
+      uint32_t there = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t w = s.words[word_of(first + j)];
+        typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+        if (half < 0) {
+          total = __builtin_amdgcn_sad_u16(w, 0u, total);
+          there |= __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(ushort2_t, w), ushort2_t{1, 1})) << j;
+        } else {
+          there |= min(w, 1u) << (j + 16 * half);
+        }
+      }
+      if (first < 0x8000 - kInf) there &= 0xffff0000u;         // -inf and the NaN's behind it
+      if (first >= kInf) there &= first == kInf ? 0x1ffffu : 0xffffu;
+      occur[b] = there;
+      if (there >> 16) largest = max(largest, 0x8000 + first + 15 - __clz((int)(there & 0xffff0000u)));
+      if (there & 0xffffu) largest = max(largest, first + 31 - __clz((int)(there & 0xffffu)));
+    }
+    if (half < 0) {
+      total = wave_total(total);
+      if (lane == 63) atomicAdd(&s.total, total);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) largest = max(largest, __shfl_xor(largest, o, 64));
+    if (lane == 0) atomicMax(&s.max_key, largest);
+    __syncthreads();
+    max_key = s.max_key;
+  };
+  Scale sc = {0.0, 0.0, top};
+  const bool least_on = set.min_p > 0.0f;
+  const double least_t = least_on ? -log2((double)fminf(set.min_p, 1.0f)) * kPerOctave : -1.0;
+  // A weight times a count: below 2^63, the count below 2^24.
+  auto times = [](uint64_t w, uint32_t c) __attribute__((always_inline)) {
+    return (uint64_t)(uint32_t)w * c + ((uint64_t)((uint32_t)(w >> 32) * c) << 32);
+  };
+  // Sums of the thread's blocks; keys beyond the last bin have no weight and are not counted.
+  uint64_t own[4] = {0, 0, 0, 0}, least = 0;
+  uint32_t own_n[4] = {0, 0, 0, 0};
+  auto sums = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      uint64_t mass = 0;
+      uint32_t n = 0;
+#pragma unroll 1
+      for (uint32_t left = b < 2 ? occur[b] & 0xffffu : occur[b - 2] >> 16; left; left &= left - 1) {
+        const int k = 16 * (tid + 1024 * b) + __ffs((int)left) - 1;
+        const double t = bins_below(sc, value(k));
+        if (t < (double)kBins) {
+          const uint32_t c = counter(k);
+          const uint64_t m = times(weight(sc, s.table, placed(t)), c);
+          mass += m;
+          n += c;
+          least += t <= least_t ? m : 0;
+        }
+      }
+      own[b] += mass;
+      own_n[b] += n;
+    }
+  };
+  const bool greedy = !(set.T > 0.0f);
+  look();
+  const bool wide = s.total != (uint32_t)vocab;
+  if (wide) {
+    __syncthreads();
+    if (tid == 0) s.max_key = -1;
+    half = 1;
+  }
+#pragma unroll 1
+  for (;;) {               // once, or the upper half's and the lower half's keys one after the other
+    if (wide) {
+      count(half);
+      look();
+    }
+    if (max_key >= 0 && !greedy) {
+      sc = scale_of(value(max_key), set.T, top);
+      sums();
+    }
+    if (half <= 0) break;
+    __syncthreads();
+    half = 0;
+  }
+  if (least_on) {
+    least = wave_total(least);
+    if (lane == 63 && least) atomicAdd((unsigned long long *)&s.least, (unsigned long long)least);
+  }
+  __syncthreads();
+  int64_t chosen = -1;
+  float lp = -INFINITY;
+  int key = max_key;
+  uint32_t place = 0;
+  if (max_key >= 0 && greedy) lp = 0.0f;
+  if (max_key >= 0 && !greedy) {
+    // sums in front of this thread's blocks, from the top: those behind them in the keys' order, the upper blocks first
+    uint64_t before[4], total = 0;
+    uint32_t before_n[4], total_n = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      before[b] = wave_scan(own[b]);
+      before_n[b] = wave_scan(own_n[b]);
+      if (lane == 63) {
+        s.part_mass[b][wave] = before[b];
+        s.part_count[b][wave] = before_n[b];
+      }
+    }
+    __syncthreads();
+    const uint64_t least_sum = s.least;
+#pragma unroll
+    for (int b = 3; b >= 0; --b) {
+      const uint64_t m = wave_scan(lane < 16 ? s.part_mass[b][lane & 15] : 0);
+      const uint32_t c = wave_scan(lane < 16 ? s.part_count[b][lane & 15] : 0u);
+      auto upto = [&](int w) __attribute__((always_inline)) {
+        return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), w) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)m, w);
+      };
+      const int w = wave ? wave - 1 : 0;
+      total += upto(15);
+      total_n += (uint32_t)__builtin_amdgcn_readlane((int)c, 15);
+      before[b] = total - before[b] - (wave ? upto(w) : 0);
+      before_n[b] = total_n - before_n[b] - (wave ? (uint32_t)__builtin_amdgcn_readlane((int)c, w) : 0);
+    }
+    const bool by_k = set.top_k > 0 && (uint32_t)set.top_k < total_n, by_p = set.top_p < 1.0f;
+    const uint64_t largest = 1ull << top, least_mass = least_on ? larger(least_sum, largest) : ~0ull;
+    uint64_t run = total;                // of top-k's run, then of the shortest one
+#pragma unroll 1
+    for (int question = by_k ? 0 : by_p ? 1 : 2; question < 3; ++question) {
+      if (question == 1 && !by_p) continue;
+      if (question == 2) run = lesser(run, least_mass);
+      const bool by_count = question == 0;
+      const uint64_t target = by_count ? (uint64_t)(set.top_k - 1) : question == 1 ? top_p_target(set.top_p, run) : token_target(u, run);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint64_t f = by_count ? before_n[b] : before[b], o = by_count ? own_n[b] : own[b];
+        if (f <= target && target < f + o) {
+          s.group = 1024 * b + tid;
+          s.base_mass = before[b];
+          s.base_count = before_n[b];
+        }
+      }
+      __syncthreads();
+      const int group = s.group;
+      if (wide && (group >> 11) != half) {
+        half = group >> 11;
+        count(half);
+      }
+      if (wave == 0) {                   // the block's keys from the top
+        const int k = group * 16 + 15 - (lane & 15);
+        const double t = bins_below(sc, value(k));
+        const bool in = lane < 16 && allowed(k) && t < (double)kBins;
+        const uint32_t c = in ? counter(k) : 0;
+        const uint64_t w = weight(sc, s.table, in ? placed(t) : 0.0), m = times(w, c);
+        const uint64_t front = s.base_mass + wave_scan(m) - m;
+        const uint32_t front_n = s.base_count + wave_scan(c) - c;
+        const uint64_t f = by_count ? front_n : front, over = target - f;
+        if (f <= target && over < (by_count ? (uint64_t)c : m)) {
+          uint64_t n = over;
+          if (!by_count) {               // the quotient of two integers below 2^62 that is below 2^24
+            n = (uint64_t)((double)over / (double)w);
+            if (n * w > over) --n;
+            else if ((n + 1) * w <= over) ++n;
+          }
+          s.key = k;
+          s.place = (uint32_t)n;
+          s.upto = front + (n + 1) * w;
+        }
+      }
+      __syncthreads();
+      if (question < 2) run = s.upto;
+    }
+    key = s.key;
+    place = s.place;
+    lp = (float)(-placed(bins_below(sc, value(key))) * (0.693147180559945309417 / kPerOctave) - log(ldexp((double)run, -top)));
+  }
+  if (key >= 0) {
+    // The place-th occurrence of the value: the elements in front of the pieces, sixteen runs of pieces, the rest.
+    const uint32_t bits = key & 0x8000 ? key & 0x7fff : ~key & 0xffff;
+    const uint32_t seen = bits == 0 ? 0x7fff7fffu : ~0u, pair = bits * 0x10001u;        // (0 in both its forms)
+    const int run = (row.pieces + 15) / 16, begin = min(wave * run, row.pieces), end = min(begin + run, row.pieces);
+    auto matches = [&](u32x4 v) __attribute__((always_inline)) {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = (v[e] & seen) ^ pair;
+        hits |= (x & 0xffffu) == 0 ? 1u << (2 * e) : 0u;
+        hits |= (x >> 16) == 0 ? 2u << (2 * e) : 0u;
+      }
+      return hits;
+    };
+    uint32_t n = 0;
+    int first = 0x7fffffff;
+    for (int i0 = begin; i0 < end; i0 += U * 64) {
+      u32x4 v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * 64 + lane;
+        v[k] = row.piece(i < end ? i : begin);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * 64 + lane;
+        const uint32_t hits = i < end ? matches(v[k]) : 0;
+        if (hits) {
+          n += __popc(hits);
+          first = min(first, row.head + i * 8 + __ffs(hits) - 1);
+        }
+      }
+    }
+    n = wave_scan(n);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+    if (lane == 63) {
+      s.seg_count[1 + wave] = n;
+      s.seg_first[1 + wave] = first;
+    }
+    const int tail = row.head + row.pieces * 8, n_tail = vocab - tail;
+    uint64_t ends = 0;                   // which of these elements match (at most seven; wavefronts 0 and 1)
+    if (wave < 2) {
+      const int m = wave == 0 ? row.head : n_tail, i = wave == 0 ? lane : tail + lane;
+      const uint32_t x = lane < m ? reinterpret_cast<const uint16_t *>(row.p)[i] : 0;
+      ends = __ballot(lane < m && ((x & seen & 0xffffu) == bits));
+      if (lane == 0) s.seg_count[17 * wave] = __popcll(ends);
+    }
+    __syncthreads();
+    const uint32_t of = lane < 18 ? s.seg_count[lane] : 0, behind = wave_scan(of);
+    const uint64_t mine = __ballot(lane < 18 && behind > place);
+    const int seg = mine ? __ffsll((unsigned long long)mine) - 1 : 17;
+    uint32_t left = place - (uint32_t)__shfl((int)(behind - of), seg, 64);
+    if (seg == 0 || seg == 17) {
+      if (wave == (seg == 17)) {
+        for (uint32_t q = 0; q < left; ++q) ends &= ends - 1;
+        if (lane == 0) s.index = (seg == 0 ? 0 : tail) + __ffsll((unsigned long long)ends) - 1;
+      }
+    } else if (seg == 1 + wave) {
+      if (left == 0) {
+        if (lane == 0) s.index = s.seg_first[seg];
+      } else {
+        for (int i0 = begin; i0 < end; i0 += 64) {
+          const int i = i0 + lane;
+          uint32_t hits = i < end ? matches(row.piece(i)) : 0;
+          const uint32_t own = __popc(hits), upto = wave_scan(own), all = (uint32_t)__shfl((int)upto, 63, 64);
+          if (left < all) {
+            if (upto - own <= left && left < upto) {
+              for (uint32_t q = upto - own; q < left; ++q) hits &= hits - 1;
+              s.index = row.head + i * 8 + __ffs(hits) - 1;
+            }
+            break;
+          }
+          left -= all;
+        }
+      }
+    }
+    __syncthreads();
+    chosen = s.index;
+  }
+  if (tid == 0) {
+    token[r] = chosen;
+    if (logprob) logprob[r] = lp;
+    if (adv.counter_a) {
+      adv.counter_a[0] = was_a + 1;
+      if (adv.word) rdkv_host_word(adv.word, 0, adv.tag_base + (uint32_t)(was_a + 1), (int32_t)chosen);
+    }
+    if (adv.counter_b) adv.counter_b[0] = was_b + 1;
+  }
+  if (tid < adv.n_counts) adv.counts[tid] += 1;
+}
+
 int weight_bits(int vocab) {             // of the largest weight: all of them together stay below 2^63
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
@@ -720,37 +1166,51 @@ int weight_bits(int vocab) {             // of the largest weight: all of them t
 }
 
 // Slices of a row: about four workgroups per compute unit over the rows, none of less than 256 pieces.
-int slices_of(int rows, int vocab, int dtype) {
-  const int pieces = vocab / (dtype == RDKV_DTYPE_F32 ? 4 : 8);
+int slices_of(int rows, int vocab) {
+  const int pieces = vocab / 4;
   const int want = (int)rdkv_cdiv(1024, rows), most = (int)rdkv_cdiv(pieces, 256);
   int s = want < most ? want : most;
   s = s < kMaxSlices ? s : kMaxSlices;
   return s < 1 ? 1 : s;
 }
 
-template <int dtype>
-int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set,
-                  const float *uniform, int64_t *token, float *logprob, const Advance &adv, void *workspace,
+int launch_slices(const char *fn, const float *logits, int64_t stride, int rows, int vocab, const Settings &set,
+                  const float *uniform, int64_t *token, float *logprob, const Advance &adv, RowSpace *space,
                   hipStream_t s) {
-  RowSpace *space = reinterpret_cast<RowSpace *>(workspace);
-  const int slices = slices_of(rows, vocab, dtype), top = weight_bits(vocab);
-  constexpr int size = dtype == RDKV_DTYPE_F32 ? 4 : 2;
+  constexpr int F32 = RDKV_DTYPE_F32;
+  const int slices = slices_of(rows, vocab), top = weight_bits(vocab);
   for (int r = 0; r < rows; r += 65535) {                  // (a grid's second dimension)
     const int n = rows - r < 65535 ? rows - r : 65535;
-    const void *from = reinterpret_cast<const char *>(logits) + (int64_t)r * stride * size;
+    const float *from = logits + (int64_t)r * stride;
     Settings part = set;
     if (part.temperature) part.temperature += r;
     if (part.top_k) part.top_k += r;
     if (part.top_p) part.top_p += r;
     if (part.min_p) part.min_p += r;
-    hipLaunchKernelGGL(sample_max_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
+    hipLaunchKernelGGL(sample_max_kernel<F32>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
     RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_bins_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
+    hipLaunchKernelGGL(sample_bins_kernel<F32>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
     RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_choose_kernel<dtype>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
+    hipLaunchKernelGGL(sample_choose_kernel<F32>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
                        uniform + r, space + r, token + r, logprob ? logprob + r : nullptr, adv);
     RDKV_CHECK_LAUNCH(fn);
   }
+  return RDKV_OK;
+}
+int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, int dtype, const Settings &set,
+                  const float *uniform, int64_t *token, float *logprob, const Advance &adv, void *workspace,
+                  hipStream_t s) {
+  if (dtype == RDKV_DTYPE_F32)
+    return launch_slices(fn, reinterpret_cast<const float *>(logits), stride, rows, vocab, set, uniform, token, logprob, adv,
+                         reinterpret_cast<RowSpace *>(workspace), s);
+  const int top = weight_bits(vocab);
+  if (dtype == RDKV_DTYPE_F16)
+    hipLaunchKernelGGL(sample_values_kernel<RDKV_DTYPE_F16>, dim3(rows), dim3(1024), sizeof(Values), s, logits, stride, vocab, top, set,
+                       uniform, token, logprob, adv);
+  else
+    hipLaunchKernelGGL(sample_values_kernel<RDKV_DTYPE_BF16>, dim3(rows), dim3(1024), sizeof(Values), s, logits, stride, vocab, top, set,
+                       uniform, token, logprob, adv);
+  RDKV_CHECK_LAUNCH(fn);
   return RDKV_OK;
 }
 
@@ -763,23 +1223,21 @@ int sample(const char *fn, const void *logits, int64_t stride, int rows, int voc
   if (rows == 0) return RDKV_OK;
   RDKV_REQUIRE(logits && uniform && token, "%s: null pointer", fn);
   RDKV_REQUIRE(stride >= 0 && ((uintptr_t)logits % (dtype == RDKV_DTYPE_F32 ? 4 : 2)) == 0, "%s: bad rows", fn);
-  if (!workspace || workspace_bytes < rdkv_sample_workspace_bytes(rows) || (uintptr_t)workspace % 16 != 0) {
-    rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)rdkv_sample_workspace_bytes(rows));
+  const int64_t need = rdkv_sample_workspace_bytes(rows, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0)) {
+    rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
     return RDKV_EWORKSPACE;
   }
   const Settings set = {sampling->temperature, sampling->top_k, sampling->top_p, sampling->min_p,
                         sampling->temperature_value, sampling->top_k_value, sampling->top_p_value, sampling->min_p_value};
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == RDKV_DTYPE_F32)
-    return launch_sample<RDKV_DTYPE_F32>(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, workspace, s);
-  if (dtype == RDKV_DTYPE_F16)
-    return launch_sample<RDKV_DTYPE_F16>(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, workspace, s);
-  return launch_sample<RDKV_DTYPE_BF16>(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, workspace, s);
+  return launch_sample(fn, logits, stride, rows, vocab, dtype, set, uniform, token, logprob, adv, workspace, (hipStream_t)stream);
 }
 
 }  // namespace
 
-RDKV_API int64_t rdkv_sample_workspace_bytes(int rows) { return rows <= 0 ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace); }
+RDKV_API int64_t rdkv_sample_workspace_bytes(int rows, int dtype) {
+  return rows <= 0 || dtype != RDKV_DTYPE_F32 ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace);
+}
 
 RDKV_API int rdkv_sample_rows(const void *logits, int64_t stride_row, int rows, int vocab, int dtype,
                               const float *uniform, const RdkvSampling *sampling, int64_t *token, float *logprob,

@@ -91,12 +91,12 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
             return token, logprob
         uniform = uniform.contiguous()
         lib = _lib.load()
-        need = lib.rdkv_sample_workspace_bytes(B)
+        need = lib.rdkv_sample_workspace_bytes(B, _lib.DTYPE_CODE[rows.dtype])
         # (the call's own, so that graphs that hold such calls may replay side by side)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.rdkv_sample_rows(rows.data_ptr(), rows.stride(0), B, vocab, _lib.DTYPE_CODE[rows.dtype],
                                         uniform.data_ptr(), ctypes.addressof(s), token.data_ptr(), logprob.data_ptr(),
-                                        ws.data_ptr(), need, _lib.stream_of(dev)))
+                                        _lib.ptr(ws), need, _lib.stream_of(dev)))
     return token, logprob
 
 
@@ -115,10 +115,10 @@ def _sample_advance(logits: torch.Tensor, token: torch.Tensor, sampling: Samplin
     lib = _lib.load()
     with torch.cuda.device(dev):
         s, _ = _settings(dev, 1, sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
-        need = lib.rdkv_sample_workspace_bytes(1)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        need = lib.rdkv_sample_workspace_bytes(1, _lib.DTYPE_CODE[row.dtype])
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.rdkv_sample_advance(
             row.data_ptr(), row.numel(), _lib.DTYPE_CODE[row.dtype], uniforms.data_ptr(), uniforms.numel(),
             write_row.data_ptr(), ctypes.addressof(s), token.data_ptr(), position.data_ptr(), write_row.data_ptr(),
             _lib.ptr(n_new), 0 if n_new is None else n_new.numel(), word.ptr if word is not None else None,
-            word.tag_base if word is not None else 0, ws.data_ptr(), need, _lib.stream_of(dev)))
+            word.tag_base if word is not None else 0, _lib.ptr(ws), need, _lib.stream_of(dev)))

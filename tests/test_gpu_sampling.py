@@ -110,6 +110,29 @@ def test_flat_rows(V, spread):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_values_that_occur_very_often(dtype):
+    """More occurrences of one value than 16 bits count: of a positive one, a negative one, zeros of both signs, the lowest
+    value as a mask; next to rows that stay just below."""
+    require_gpu()
+    V = 140_003
+    g = torch.Generator().manual_seed(77)
+    x = torch.randn(8, V, generator=g)
+    often = torch.rand(8, V, generator=g) < 0.7
+    for row, v in enumerate([2.5, -1.5, 0.0, -0.0, torch.finfo(dtype).min, 0.0]):
+        x[row, often[row]] = v
+    x[5, ::2] = torch.where(x[5, ::2] == 0, -0.0, x[5, ::2])
+    x[6] = 0.25
+    x[6, 65535:] = -3.0 - torch.rand(V - 65535, generator=g)
+    x[7] = -0.25
+    x[7, 65536:] = -3.0 - torch.rand(V - 65536, generator=g)
+    u = torch.rand(8, generator=g).numpy()
+    for setting in (dict(), dict(T=0.0), dict(k=60_000), dict(p=0.5, T=3.0), dict(k=100_000, p=0.9, min_p=0.1, T=2.0)):
+        check(x.to(dtype), u, **setting, what=str(setting))
+        check(x.to(dtype), u[::-1].copy(), **setting, what=str(setting))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_masks_infinities_and_no_numbers(dtype):
     require_gpu()
     V = 3001
@@ -278,21 +301,21 @@ def test_refusals_of_the_c_interface():
     lib = _lib.load()
     one = 1 << 20                    # a pointer that is looked at, never followed
     s = _lib.RdkvSampling(temperature_value=1.0, top_p_value=1.0)
-    need = lib.rdkv_sample_workspace_bytes(2)
-    assert need > 0 and lib.rdkv_sample_workspace_bytes(0) == 0 and lib.rdkv_sample_workspace_bytes(-3) == 0
+    need = lib.rdkv_sample_workspace_bytes(2, 0)
+    assert need > 0 and lib.rdkv_sample_workspace_bytes(0, 0) == lib.rdkv_sample_workspace_bytes(-3, 0) == lib.rdkv_sample_workspace_bytes(2, 1) == 0
 
-    def rows(logits=one, stride=64, n=2, vocab=64, dt=1, u=one, settings=ctypes.addressof(s), token=one, ws=one, nb=need):
+    def rows(logits=one, stride=64, n=2, vocab=64, dt=0, u=one, settings=ctypes.addressof(s), token=one, ws=one, nb=need):
         return lib.rdkv_sample_rows(logits, stride, n, vocab, dt, u, settings, token, None, ws, nb, None)
 
     for bad in (dict(n=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(dt=3), dict(settings=None), dict(logits=None), dict(u=None),
-                dict(token=None), dict(stride=-64), dict(logits=one + 1), dict(logits=one + 2, dt=0)):
+                dict(token=None), dict(stride=-64), dict(logits=one + 1, dt=1), dict(logits=one + 2)):
         assert rows(**bad) == _lib.RDKV_EINVAL, bad
     for bad in (dict(ws=None), dict(nb=need - 1), dict(ws=one + 8)):
         assert rows(**bad) == _lib.RDKV_EWORKSPACE, bad
     assert rows(n=0) == _lib.RDKV_OK
 
     def advance(n_uniform=4, index=one, counter=one, counts=None, n_counts=0, word=None):
-        return lib.rdkv_sample_advance(one, 64, 1, one, n_uniform, index, ctypes.addressof(s), one, counter, None, counts, n_counts, word,
+        return lib.rdkv_sample_advance(one, 64, 0, one, n_uniform, index, ctypes.addressof(s), one, counter, None, counts, n_counts, word,
                                        0, None, 0, None)
 
     for bad in (dict(n_uniform=0), dict(index=None), dict(n_counts=1025, counts=one), dict(n_counts=1), dict(counter=None, word=one)):
