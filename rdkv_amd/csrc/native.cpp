@@ -14,6 +14,7 @@
 #include <ATen/ops/cat.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
+#include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
 #include <initializer_list>
@@ -31,7 +32,9 @@ namespace {
   X(rdkv_pack_layers_k_minmax) X(rdkv_pack_layer_v_rows) X(rdkv_pack_layer_tables) X(rdkv_pack_layer_k_rows)     \
   X(rdkv_decode_fused) X(rdkv_decode_fused_zone_c) X(rdkv_decode_fused_workspace_bytes)                           \
   X(rdkv_unpack_layer) X(rdkv_stream_plan_layer) X(rdkv_pack_layer) X(rdkv_plan_layers)                                                           \
-  X(rdkv_select_layer_start) X(rdkv_pack_layers_stream)
+  X(rdkv_select_layer_start) X(rdkv_pack_layers_stream)                                                          \
+  X(rdkv_w4_linear) X(rdkv_w4_linear_workspace_bytes) X(rdkv_w4_linear_norm) X(rdkv_w4_linear_silu)              \
+  X(rdkv_sample_rows) X(rdkv_sample_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   RDKV_NATIVE_FUNCTIONS(X)
@@ -745,6 +748,165 @@ PyObject *dense_layer(PyObject *const *a, Py_ssize_t) {
   return Ref(PyTuple_Pack(3, k.o, v.o, additive.o)).release();
 }
 
+// ---- products with 4-bit weights (weight_quant) ------------------------------------------------------------------------
+// A quantized matrix as its fields, from argument `i` on: codes, scales, N, K, group, type.
+struct Quantized {
+  const at::Tensor &codes, &scales;
+  int64_t N, K, group, dtype;
+  Quantized(PyObject *const *a, int i)
+      : codes(tensor(a[i])), scales(tensor(a[i + 1])), N(integer(a[i + 2])), K(integer(a[i + 3])), group(integer(a[i + 4])),
+        dtype(integer(a[i + 5])) {
+    plain(codes.is_cuda() && scales.device() == codes.device() && N > 0 && K > 0);
+    plain(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kInt && codes.is_contiguous() && scales.is_contiguous());
+  }
+  const uint32_t *words() const { return reinterpret_cast<const uint32_t *>(scales.data_ptr()); }
+  bool type(const at::Tensor &t) const { return t.device() == codes.device() && dtype_code(t) == dtype; }
+  // a row of K values
+  bool row(const at::Tensor &t) const { return type(t) && t.dim() >= 1 && t.size(-1) == K && t.numel() == K && t.stride(-1) == 1; }
+  at::Tensor bias(PyObject *o) const {
+    if (o == Py_None) return at::Tensor();
+    const at::Tensor &b = tensor(o);
+    plain(type(b) && shape_is(b, {N}) && b.is_contiguous());
+    return b;
+  }
+  at::Tensor result(const at::Tensor &like) const {
+    std::vector<int64_t> s(like.sizes().begin(), like.sizes().end());
+    s.back() = N;
+    return at::empty(s, options(like));
+  }
+  at::TensorOptions options(const at::Tensor &like) const {
+    return at::TensorOptions().device(like.device()).dtype(dtype == RDKV_DTYPE_F16 ? at::kHalf : at::kBFloat16);
+  }
+};
+
+// x, codes, scales, N, K, group, type, bias or None, stream
+PyObject *w4_linear(PyObject *const *a, Py_ssize_t) {
+  const at::Tensor &x = tensor(a[0]);
+  const Quantized q(a, 1);
+  const at::Tensor bias = q.bias(a[7]);
+  void *stream = address(a[8]);
+  const int code = dtype_code(x);
+  plain(x.device() == q.codes.device() && (code == q.dtype || code == RDKV_DTYPE_F32));
+  plain(x.dim() >= 1 && x.size(-1) == q.K && x.stride(-1) == 1 && (x.dim() <= 2 || x.is_contiguous()));
+  const int64_t M = x.numel() / q.K, stride = x.dim() == 2 ? x.stride(0) : q.K;
+  plain(M >= 1 && M <= 1 << 20 && stride >= 0);
+  at::Tensor y, ws;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(x.device());
+    y = q.result(x);
+    const int64_t need = M == 1 && q.K <= 32768 ? 0 : lib.rdkv_w4_linear_workspace_bytes(M, q.K);
+    if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
+    rc = lib.rdkv_w4_linear(q.codes.data_ptr(), q.words(), x.data_ptr(), code, stride, data(bias), M, q.N, q.K, q.group, q.dtype,
+                            y.data_ptr(), q.N, data(ws), need, stream);
+  }
+  status(rc);
+  return wrap(y);
+}
+
+// h, delta or None, norm weight, eps, codes, scales, N, K, group, type, bias or None, stream
+PyObject *w4_norm_linear(PyObject *const *a, Py_ssize_t) {
+  const at::Tensor &h = tensor(a[0]), &norm = tensor(a[2]);
+  const at::Tensor delta = a[1] == Py_None ? at::Tensor() : tensor(a[1]);
+  const double eps = real(a[3]);
+  const Quantized q(a, 4);
+  const at::Tensor bias = q.bias(a[10]);
+  void *stream = address(a[11]);
+  plain(q.row(h) && (!delta.defined() || q.row(delta)) && q.type(norm) && shape_is(norm, {q.K}) && norm.is_contiguous() && q.K <= 32768);
+  at::Tensor y, r;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(h.device());
+    y = q.result(h);
+    if (delta.defined()) r = at::empty(h.sizes(), q.options(h));
+    rc = lib.rdkv_w4_linear_norm(q.codes.data_ptr(), q.words(), h.data_ptr(), data(delta), norm.data_ptr(), (float)eps, data(r),
+                                 data(bias), q.N, q.K, q.group, q.dtype, y.data_ptr(), stream);
+  }
+  status(rc);
+  Ref o(wrap(y));
+  if (!delta.defined()) return Ref(PyTuple_Pack(2, o.o, a[0])).release();
+  Ref s(wrap(r));
+  return Ref(PyTuple_Pack(2, o.o, s.o)).release();
+}
+
+// gate, up, codes, scales, N, K, group, type, bias or None, stream
+PyObject *w4_silu_linear(PyObject *const *a, Py_ssize_t) {
+  const at::Tensor &gate = tensor(a[0]), &up = tensor(a[1]);
+  const Quantized q(a, 2);
+  const at::Tensor bias = q.bias(a[8]);
+  void *stream = address(a[9]);
+  plain(q.row(gate) && q.row(up) && q.K <= 32768);
+  at::Tensor y;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(gate.device());
+    y = q.result(gate);
+    rc = lib.rdkv_w4_linear_silu(q.codes.data_ptr(), q.words(), gate.data_ptr(), up.data_ptr(), data(bias), q.N, q.K, q.group,
+                                 q.dtype, y.data_ptr(), stream);
+  }
+  status(rc);
+  return wrap(y);
+}
+
+// ---- sampling (sampling.sample_tokens) -------------------------------------------------------------------------------------
+// logits, uniform, temperature, top-k, top-p, min-p (numbers, or a tensor with a value per row), stream
+PyObject *sample_rows(PyObject *const *a, Py_ssize_t) {
+  const at::Tensor &logits = tensor(a[0]), &uniform = tensor(a[1]);
+  const int code = dtype_code(logits);
+  plain(logits.is_cuda() && code >= 0 && logits.dim() >= 1 && logits.stride(-1) == 1 && (logits.dim() <= 2 || logits.is_contiguous()));
+  const int64_t vocab = logits.size(-1);
+  plain(vocab >= 1 && vocab <= 1 << 24);
+  const int64_t rows = logits.numel() / vocab, stride = logits.dim() == 2 ? logits.stride(0) : vocab;
+  const at::IntArrayRef shape = logits.sizes().slice(0, logits.dim() - 1);
+  plain(rows >= 1 && rows <= 0x7fffffff && stride >= 0);
+  plain(uniform.device() == logits.device() && uniform.scalar_type() == at::kFloat && uniform.sizes() == shape && uniform.is_contiguous());
+  // a setting: whether it is a tensor of the type, else its number
+  auto setting = [&](PyObject *o, at::ScalarType type, const void **at) {
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    plain(t.device() == logits.device() && t.scalar_type() == type && t.is_contiguous() && (t.sizes() == shape || shape_is(t, {rows})));
+    *at = t.data_ptr();
+    return true;
+  };
+  auto number = [&](PyObject *o, bool share) {
+    const double v = real(o);
+    plain(v == v && (!share || (v >= 0.0 && v <= 1.0)));
+    return (float)v;
+  };
+  RdkvSampling s{};
+  const void *p[4] = {nullptr, nullptr, nullptr, nullptr};
+  if (!setting(a[2], at::kFloat, &p[0])) s.temperature_value = number(a[2], false);
+  if (!setting(a[3], at::kInt, &p[1])) {
+    plain(PyLong_Check(a[3]));
+    const int64_t k = whole(a[3]);
+    plain(k <= 0x7fffffff);
+    s.top_k_value = (int32_t)std::max<int64_t>(k, 0);
+  }
+  if (!setting(a[4], at::kFloat, &p[2])) s.top_p_value = number(a[4], true);
+  if (!setting(a[5], at::kFloat, &p[3])) s.min_p_value = number(a[5], true);
+  s.temperature = static_cast<const float *>(p[0]), s.top_k = static_cast<const int32_t *>(p[1]);
+  s.top_p = static_cast<const float *>(p[2]), s.min_p = static_cast<const float *>(p[3]);
+  void *stream = address(a[6]);
+  at::Tensor token, logprob, ws;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(logits.device());
+    const auto dev = at::TensorOptions().device(logits.device());
+    token = at::empty(shape, dev.dtype(at::kLong)), logprob = at::empty(shape, dev.dtype(at::kFloat));
+    const int64_t need = lib.rdkv_sample_workspace_bytes(rows, code);
+    if (need) ws = at::empty({need}, dev.dtype(at::kByte));
+    rc = lib.rdkv_sample_rows(logits.data_ptr(), stride, rows, vocab, code, uniform.data_ptr<float>(), &s, token.data_ptr<int64_t>(),
+                              logprob.data_ptr<float>(), data(ws), need, stream);
+  }
+  status(rc);
+  Ref t(wrap(token)), l(wrap(logprob));
+  return Ref(PyTuple_Pack(2, t.o, l.o)).release();
+}
+
 // {name: address of the function}, check
 PyObject *bind(PyObject *const *a, Py_ssize_t) {
   Library l;
@@ -775,6 +937,10 @@ PyMethodDef kMethods[] = {
     ENTRY(stream_pack, 12, "The blobs of the layers, or None."),
     ENTRY(decode_attn, 16, "(out, lse) of a decode step, or None."),
     ENTRY(dense_layer, 7, "Dense (K, V) of a packed layer, with its additive mask where one is given; or None."),
+    ENTRY(w4_linear, 9, "The product of activation rows with a 4-bit matrix, or None."),
+    ENTRY(w4_norm_linear, 12, "(product, residual row) of one row with its norm, or None."),
+    ENTRY(w4_silu_linear, 10, "The product of one row with its activation, or None."),
+    ENTRY(sample_rows, 7, "(tokens, log probabilities), or None."),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Host side of the per-layer entry points.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -72,6 +72,12 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
     0).  Each setting is a number or a tensor with one value per row, on the logits' device (and not looked
     at by the host: values out of range act as the nearest one in range, NaN as off).  NaN and -inf logits are masked; a row
     with nothing left has token -1 and log probability -inf."""
+    if logits.is_cuda:              # plain arguments: csrc/native.cpp (the checks and the launch cost 27 us interpreted)
+        if _lib.native is None:
+            _lib.load()
+        pair = _lib.native.sample_rows(logits, uniform, temperature, top_k, top_p, min_p, _lib.stream_of(logits.device))
+        if pair is not None:
+            return pair
     dev = _lib.require_device(logits, uniform)
     assert logits.dim() >= 1 and logits.dtype in _lib.DTYPE_CODE, f"logits: fp32, fp16 or bf16, got {logits.dtype}"
     shape, vocab = logits.shape[:-1], logits.shape[-1]

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from rdkv_amd import _lib, sampling
-from tests.gpu_util import DEV, require_gpu
+from tests.gpu_util import DEV, record_native, require_gpu
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 
@@ -295,6 +295,24 @@ def test_advance_matches_sample_tokens_and_moves_the_counters():
         sampling._sample_advance(logits, token, s, uniforms, pos, row, n_new)
         exp, _ = sampling.sample_tokens(logits.view(1, -1), uniforms[i:i + 1], temperature=0.8, top_k=100, top_p=0.9, min_p=0.01)
         assert int(token) == int(exp) and int(pos) == 101 + step and int(row) == step + 1 and n_new.tolist() == [2 + step] * 8
+
+
+@pytest.mark.gpu
+def test_plain_calls_take_the_native_way(monkeypatch):
+    """Plain arguments go through csrc/native.cpp, others through the general path, with the same tokens."""
+    require_gpu()
+    x, u = _logits(6, 700, F16, 12)
+    xd, ud = x.to(DEV), torch.as_tensor(u, dtype=F32).to(DEV)
+    T, k = torch.full((6,), 0.7, device=DEV), torch.full((6,), 30, dtype=torch.int32, device=DEV)
+    calls = record_native(monkeypatch)
+    token, lp = sampling.sample_tokens(xd, ud, temperature=T, top_k=k, top_p=0.9, min_p=0)
+    same = sampling.sample_tokens(xd, ud, temperature=T, top_k=30, top_p=0.9)[0]
+    assert calls.taken == ["sample_rows"] * 2 and torch.equal(same, token)
+    for args, kw in (((xd, ud), dict(temperature=T.double(), top_k=k)), ((xd, ud), dict(temperature=T, top_k=k.long())),
+                     ((xd.t().contiguous().t(), ud), dict(temperature=T, top_k=k)), ((xd, torch.stack([ud, ud], 1)[:, 0]), dict(temperature=T, top_k=k))):
+        t2, l2 = sampling.sample_tokens(*args, top_p=0.9, **kw)
+        assert torch.equal(t2, token) and torch.equal(l2, lp)
+    assert len(calls.asked) == 6 and len(calls.taken) == 2
 
 
 def test_refusals_of_the_c_interface():

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from rdkv_amd import _lib, weight_quant as wq
-from tests.gpu_util import DEV, require_gpu
+from tests.gpu_util import DEV, record_native, require_gpu
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -230,6 +230,30 @@ def test_products_on_streams_and_in_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, eager)), f"replay {rep}"
+
+
+@pytest.mark.gpu
+def test_plain_calls_take_the_native_way(monkeypatch):
+    """Plain arguments go through csrc/native.cpp, others through the general path, with the same bits."""
+    require_gpu()
+    g = torch.Generator().manual_seed(8)
+    q = wq.quantize_weight((torch.randn(50, 300, generator=g) * 0.1).to(F16).to(DEV), 32)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(F16).to(DEV)  # noqa: E731
+    x, bias, h, delta, norm, up = rnd(2, 3, 300), rnd(50), rnd(1, 300), rnd(1, 300), rnd(300), rnd(1, 300)
+    calls = record_native(monkeypatch)
+    y = wq.linear(x, q, bias)
+    n, r = wq.norm_linear(h, delta, norm, 1e-5, q, bias)
+    s = wq.silu_linear(h, up, q)
+    assert calls.taken == ["w4_linear", "w4_norm_linear", "w4_silu_linear"]
+    general = wq.linear(x.transpose(0, 1), q, bias)                   # rows that are no plain view
+    assert calls.taken[3:] == [] and calls.asked[3:] == ["w4_linear"] and torch.equal(general, y.transpose(0, 1))
+    wide = torch.stack([bias, bias], 1)[:, 0]                         # a bias of another stride
+    assert torch.equal(wq.linear(x, q, wide), y) and torch.equal(wq.norm_linear(h, delta, norm, 1e-5, q, wide)[0], n)
+    assert torch.equal(wq.silu_linear(h, up, q, torch.zeros_like(wide)), s) and len(calls.taken) == 4
+    monkeypatch.setattr(_lib, "native", type("None_", (), {"__getattr__": lambda self, name: lambda *a: None})())
+    assert torch.equal(wq.linear(x, q, bias), y)
+    n2, r2 = wq.norm_linear(h, delta, norm, 1e-5, q, bias)
+    assert torch.equal(n2, n) and torch.equal(r2, r) and torch.equal(wq.silu_linear(h, up, q), s)
 
 
 def test_refusals_of_the_c_interface():
