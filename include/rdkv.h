@@ -392,10 +392,10 @@ int rdkv_w4_pack(const uint8_t *q, int64_t q_stride_row, const void *scale, int 
 int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, int K, int group, int dtype, void *out,
                     int64_t out_stride_row, void *stream);
 /* y[m, n] = sum_k x[m, k] * W[n, k] (+ bias[n]): x [M, K] of x_dtype = `dtype`, or fp32 (rounded to `dtype` first), y [M, N]
- * and bias [N] of `dtype`; fp32 accumulation in a fixed order.  Any M, N, K.  The workspace (at most
- * rdkv_w4_linear_workspace_bytes, 16-byte aligned) is used for rows that are fp32, misaligned or no multiple of 8
- * long, unless M is 1 and K at most 32768; it may be NULL otherwise. */
-int64_t rdkv_w4_linear_workspace_bytes(int M, int K);
+ * and bias [N] of `dtype`; fp32 accumulation in a fixed order.  M up to 2^19, any N, K.  The
+ * workspace (rdkv_w4_linear_workspace_bytes on the device of the call, 16-byte aligned; 0 for one row of up to 32768
+ * elements) takes the rows in the order that the products read them in. */
+int64_t rdkv_w4_linear_workspace_bytes(int M, int N, int K);
 int rdkv_w4_linear(const void *codes, const uint32_t *scales, const void *x, int x_dtype, int64_t x_stride_row,
                    const void *bias, int M, int N, int K, int group, int dtype, void *y, int64_t y_stride_row,
                    void *workspace, int64_t workspace_bytes, void *stream);

@@ -121,7 +121,7 @@ SIGNATURES = {
     "rdkv_w4_quantize": (I, [P, L, I, I, I, I, P, P, P]),
     "rdkv_w4_pack": (I, [P, L, P, I, L, P, L, I, I, I, P, P, P]),
     "rdkv_w4_dequant": (I, [P, P, I, I, I, I, P, L, P]),
-    "rdkv_w4_linear_workspace_bytes": (L, [I, I]),
+    "rdkv_w4_linear_workspace_bytes": (L, [I, I, I]),
     "rdkv_w4_linear": (I, [P, P, P, I, L, P, I, I, I, I, I, P, L, P, L, P]),
     "rdkv_w4_linear_norm": (I, [P, P, P, P, P, F, P, P, I, I, I, I, P, P]),
     "rdkv_w4_linear_silu": (I, [P, P, P, P, P, I, I, I, I, P, P]),

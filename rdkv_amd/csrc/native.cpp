@@ -789,14 +789,14 @@ PyObject *w4_linear(PyObject *const *a, Py_ssize_t) {
   plain(x.device() == q.codes.device() && (code == q.dtype || code == RDKV_DTYPE_F32));
   plain(x.dim() >= 1 && x.size(-1) == q.K && x.stride(-1) == 1 && (x.dim() <= 2 || x.is_contiguous()));
   const int64_t M = x.numel() / q.K, stride = x.dim() == 2 ? x.stride(0) : q.K;
-  plain(M >= 1 && M <= 1 << 20 && stride >= 0);
+  plain(M >= 1 && M <= 1 << 19 && stride >= 0);
   at::Tensor y, ws;
   int rc;
   {
     Unlocked u;
     const c10::DeviceGuard guard(x.device());
     y = q.result(x);
-    const int64_t need = M == 1 && q.K <= 32768 ? 0 : lib.rdkv_w4_linear_workspace_bytes(M, q.K);
+    const int64_t need = lib.rdkv_w4_linear_workspace_bytes((int)M, q.N, q.K);
     if (need) ws = at::empty({need}, x.options().dtype(at::kByte));
     rc = lib.rdkv_w4_linear(q.codes.data_ptr(), q.words(), x.data_ptr(), code, stride, data(bias), M, q.N, q.K, q.group, q.dtype,
                             y.data_ptr(), q.N, data(ws), need, stream);

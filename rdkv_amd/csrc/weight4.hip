@@ -30,10 +30,14 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = 1024;
 constexpr float kSmallestScale = 0x1p-120f;      // below it a group counts as all zeros (its scale stays an ordinary number)
 
+// Sixteen bytes at any address of a 16-bit element.
+struct __attribute__((packed, aligned(2))) Loose { u32x4 v; };
+__device__ __forceinline__ u32x4 load_loose(const uint16_t *p) { return reinterpret_cast<const Loose *>(p)->v; }
 __device__ __forceinline__ u32x4 load_stream(const u32x4 *p) { return __builtin_nontemporal_load(p); }
 
 template <int dtype>
@@ -52,55 +56,90 @@ __device__ __forceinline__ int field_shift(int j) { return 4 * (j >> 1) + 16 * (
 
 // ---- quantize / pack / dequantize: a wavefront per tile ------------------------------------------
 
-struct TileAt { int64_t tile; int64_t row; int lane, c; int64_t col0; };
-__device__ __forceinline__ TileAt tile_at(int64_t n_tiles_k) {
+struct TileAt { int64_t tile, row; int lane, c, col0; };
+__device__ __forceinline__ TileAt tile_at(uint32_t n_tiles_k) {
   TileAt t;
   t.lane = threadIdx.x & 63;
   t.c = t.lane >> 4;
-  t.tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  t.row = (t.tile / n_tiles_k) * kTileRows + (t.lane & 15);
-  t.col0 = (t.tile % n_tiles_k) * kTileCols;
+  const uint32_t tile = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // below 2^31 + 3
+  t.tile = tile;
+  t.row = (int64_t)(tile / n_tiles_k) * kTileRows + (t.lane & 15);
+  t.col0 = (int)(tile % n_tiles_k * kTileCols);        // (below K, which is at most 2^31 - 256)
   return t;
 }
 
+// Eight elements without the first n, zeros behind the others.
+__device__ __forceinline__ u32x4 drop_front(u32x4 v, int n) {
+  if (n <= 0) return v;
+  if (n & 4) v = u32x4{v[2], v[3], 0, 0};
+  if (n & 2) v = u32x4{v[1], v[2], v[3], 0};
+  if (n & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+  return n >= 8 ? u32x4{0, 0, 0, 0} : v;
+}
+// A mask of the first n of a dword's eight fields: an even field j lies at bit 2 j, an odd one at 2 (j - 1) + 16.
+__device__ __forceinline__ uint32_t fields_below(int n) {
+  if (n <= 0) return 0u;
+  if (n >= 8) return ~0u;
+  return ((1u << (4 * ((n + 1) >> 1))) - 1) | ((1u << (4 * (n >> 1))) - 1) << 16;
+}
+
 // The value range of a group takes in zero, so that a zero weight stays zero and the zero point lies in
-// 0 .. 15; divisions are the correctly rounded ones and nothing is contracted, so the codes are those of the
+// 0 .. 15; quotients are the correctly rounded ones and nothing is contracted, so the codes are those of the
 // expressions rint(w / s) + z.  A group that holds a NaN or an infinity has scale NaN: every product with it is NaN.
+// One pass: 2 bytes read and 0.53 written for a weight (groups of 128).  28672 x 4096 fp16: 53 us, 5.6 TB/s; with a division
+// for each weight that might lie between two codes it took 76.
 template <int dtype, int GPC>
 __global__ void __launch_bounds__(256)
-w4_quantize_kernel(const uint16_t *__restrict__ W, int64_t w_stride_row, int N, int K, int aligned, int64_t n_tiles_k,
-                   int64_t n_tiles, u32x4 *__restrict__ codes, uint32_t *__restrict__ scales) {
+w4_quantize_kernel(const uint16_t *__restrict__ W, int64_t w_stride_row, int N, int K, uint32_t n_tiles_k,
+                   uint32_t n_tiles, u32x4 *__restrict__ codes, uint32_t *__restrict__ scales) {
 #pragma clang fp contract(off)
   const TileAt t = tile_at(n_tiles_k);
   if (t.tile >= n_tiles) return;
-  float v[4][8];
-  const uint16_t *src = W + t.row * w_stride_row;
+  // (Read in the layout's lanes, 64 bytes of a row at a time: rows of 256 bytes turned through LDS took 59 us where this
+  // takes 53.)
+  u32x4 v[4];
+  const uint16_t *src = W + min(t.row, (int64_t)N - 1) * w_stride_row;      // (rows behind the matrix: not stored)
+  if (K >= 8) {
 #pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    const int64_t k = t.col0 + 32 * d + 8 * t.c;
-    if (t.row < N && aligned && k + 8 <= K) {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(src + k);
+    for (int d = 0; d < 4; ++d) v[d] = load_loose(src + min(t.col0 + 32 * d + 8 * t.c, K - 8));
+    if (t.col0 + kTileCols > K) {        // pieces over the end were read from column K - 8 on
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[d][j] = load16<dtype>((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[d][j] = t.row < N && k + j < K ? load16<dtype>(src[k + j]) : 0.0f;
+      for (int d = 0; d < 4; ++d) v[d] = drop_front(v[d], t.col0 + 32 * d + 8 * t.c - (K - 8));
     }
+  } else {
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 32 * d + 8 * t.c + 2 * i;
+        v[d][i] = (k < K ? src[k] : 0u) | (k + 1 < K ? (uint32_t)src[k + 1] << 16 : 0u);
+      }
   }
   constexpr int DPG = 4 / GPC;           // dwords of a lane per group
+  constexpr uint16_t kInfinite = dtype == RDKV_DTYPE_F16 ? 0x7c00 : 0x7f80;
+  auto weight = [&](int d, int j) __attribute__((always_inline)) {
+    const uint32_t pair = v[d][j >> 1];
+    return load16<dtype>((uint16_t)(pair >> (16 * (j & 1))));
+  };
   u32x4 out;
 #pragma unroll
   for (int g = 0; g < GPC; ++g) {
     float lo = 0.0f, hi = 0.0f;
-    bool bad = false;
+    u16x2 size = {0, 0};
 #pragma unroll
-    for (int d = g * DPG; d < (g + 1) * DPG; ++d)
+    for (int d = g * DPG; d < (g + 1) * DPG; ++d) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        lo = fminf(lo, v[d][j]);
-        hi = fmaxf(hi, v[d][j]);
-        bad |= !(fabsf(v[d][j]) < INFINITY);
+        lo = fminf(lo, weight(d, j));
+        hi = fmaxf(hi, weight(d, j));
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = v[d][i] & 0x7fff7fffu;
+        size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2, pair));
+      }
+    }
+    bool bad = size[0] >= kInfinite || size[1] >= kInfinite;
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) {   // the four lanes that share the row
       lo = fminf(lo, __shfl_xor(lo, o, 64));
@@ -110,23 +149,47 @@ w4_quantize_kernel(const uint16_t *__restrict__ W, int64_t w_stride_row, int N, 
     float s = word_scale(scale_word((hi - lo) / 15.0f, 0));
     if (!(s < INFINITY) || bad) s = __builtin_nanf("");
     if (s < kSmallestScale) s = 1.0f;
-    // (the clamps come last and take a NaN to 0: a group whose scale is NaN has zero codes)
-    const float z = fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f);
+    // Correctly rounded quotients without a division for each: q = v * (1 / s) is within a few ulp, its remainder v - q s is
+    // exact, and q + (v - q s) (1 / s) before its rounding is within 2^-22 ulp of v / s, which, s having 20 bits, stays
+    // 2^-21 ulp away from the middle of two fp32 numbers.  (Not where the remainder could be subnormal.)
+    const float inv = 1.0f / s;
+    auto quotient = [&](float w) __attribute__((always_inline)) {
+      const float q = w * inv;
+      return __builtin_fmaf(__builtin_fmaf(-q, s, w), inv, q);
+    };
+    const bool tiny = dtype == RDKV_DTYPE_BF16 && s < 0x1p-60f;
+    // Added to 1.5 * 2^23, a quotient is rounded to a whole number in the low bits, ties to even; after the clamp the bits of
+    // eight of them are shifted and summed, and what they hold beside the codes is a constant.  (The clamp takes a NaN to
+    // the lower end: a group whose scale is NaN has zero codes.)
+    constexpr float kWhole = 0x1.8p23f;
+    const float z = fminf(fmaxf(rintf(tiny ? -lo / s : quotient(-lo)), 0.0f), 15.0f);
+    const float from = kWhole - z, to = from + 15.0f;
+    const uint32_t beside = __float_as_uint(from) * 0x11111111u;
 #pragma unroll
     for (int d = g * DPG; d < (g + 1) * DPG; ++d) {
       uint32_t w = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = fminf(fmaxf(rintf(v[d][j] / s) + z, 0.0f), 15.0f);
-        if (t.col0 + 32 * d + 8 * t.c + j < K) w |= (uint32_t)q << field_shift(j);
+      for (int j = 0; j < 8; ++j) w += __float_as_uint(fminf(fmaxf(quotient(weight(d, j)) + kWhole, from), to)) << field_shift(j);
+      out[d] = w - beside;
+    }
+    if (tiny) {
+#pragma unroll
+      for (int d = g * DPG; d < (g + 1) * DPG; ++d) {
+        uint32_t w = 0;
+        for (int j = 0; j < 8; ++j) w |= (uint32_t)fminf(fmaxf(rintf(weight(d, j) / s) + z, 0.0f), 15.0f) << field_shift(j);
+        out[d] = w;
       }
-      out[d] = t.row < N ? w : 0u;
     }
     if (t.c == 0) {
-      const bool there = t.row < N && t.col0 + (int64_t)g * DPG * 32 < K;
+      const bool there = t.row < N && (int64_t)t.col0 + g * DPG * 32 < K;
       scales[(t.tile * GPC + g) * 16 + (t.lane & 15)] = there ? scale_word(s, (uint32_t)z) : 0u;
     }
   }
+  if (t.col0 + kTileCols > K) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) out[d] &= fields_below(K - t.col0 - 32 * d - 8 * t.c);
+  }
+  if (t.row >= N) out = u32x4{0, 0, 0, 0};
   codes[t.tile * 64 + t.lane] = out;
 }
 
@@ -135,7 +198,7 @@ template <int GPC>
 __global__ void __launch_bounds__(256)
 w4_pack_kernel(const uint8_t *__restrict__ src, int64_t src_stride_row, const void *__restrict__ scale, int scale_dtype,
                int64_t scale_stride_row, const uint8_t *__restrict__ zero, int64_t zero_stride_row, int N, int K,
-               int64_t n_tiles_k, int64_t n_tiles, u32x4 *__restrict__ codes, uint32_t *__restrict__ scales) {
+               uint32_t n_tiles_k, uint32_t n_tiles, u32x4 *__restrict__ codes, uint32_t *__restrict__ scales) {
   const TileAt t = tile_at(n_tiles_k);
   if (t.tile >= n_tiles) return;
   u32x4 out;
@@ -144,7 +207,7 @@ w4_pack_kernel(const uint8_t *__restrict__ src, int64_t src_stride_row, const vo
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int64_t k = t.col0 + 32 * d + 8 * t.c + j;
+      const int k = t.col0 + 32 * d + 8 * t.c + j;
       const uint32_t q = t.row < N && k < K ? src[t.row * src_stride_row + k] & 15u : 0u;
       w |= q << field_shift(j);
     }
@@ -152,9 +215,9 @@ w4_pack_kernel(const uint8_t *__restrict__ src, int64_t src_stride_row, const vo
   }
   codes[t.tile * 64 + t.lane] = out;
   if (t.c < GPC) {                       // lane 16 g + n: group g of row n
-    const int64_t group = t.col0 / (kTileCols / GPC) + t.c;
+    const int group = t.col0 / (kTileCols / GPC) + t.c;
     uint32_t word = 0;
-    if (t.row < N && group * (kTileCols / GPC) < K) {
+    if (t.row < N && group * (int64_t)(kTileCols / GPC) < K) {
       const float s = rdkv_load_as_float(scale, scale_dtype, t.row * scale_stride_row + group);
       word = scale_word(s, zero ? zero[t.row * zero_stride_row + group] & 15u : 8u);
     }
@@ -164,8 +227,8 @@ w4_pack_kernel(const uint8_t *__restrict__ src, int64_t src_stride_row, const vo
 
 template <int dtype, int GPC>
 __global__ void __launch_bounds__(256)
-w4_dequant_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, int N, int K, int aligned,
-                  int64_t n_tiles_k, int64_t n_tiles, uint16_t *__restrict__ out, int64_t out_stride_row) {
+w4_dequant_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, int N, int K,
+                  uint32_t n_tiles_k, uint32_t n_tiles, uint16_t *__restrict__ out, int64_t out_stride_row) {
   const TileAt t = tile_at(n_tiles_k);
   if (t.tile >= n_tiles || t.row >= N) return;
   const u32x4 q = codes[t.tile * 64 + t.lane];
@@ -174,7 +237,7 @@ w4_dequant_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ 
   for (int d = 0; d < 4; ++d) {
     const uint32_t word = scales[(t.tile * GPC + d * GPC / 4) * 16 + (t.lane & 15)];
     const float s = word_scale(word), z = (float)word_zero(word);
-    const int64_t k = t.col0 + 32 * d + 8 * t.c;
+    const int k = t.col0 + 32 * d + 8 * t.c;
     uint16_t h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -182,11 +245,11 @@ w4_dequant_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ 
       const float v = ((float)((q[d] >> field_shift(j)) & 15u) - z) * s;
       h[j] = dtype == RDKV_DTYPE_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : rdkv_float_to_bf16_bits(v);
     }
-    if (aligned && k + 8 <= K) {
+    if (k + 8 <= K) {
       u32x4 w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-      *reinterpret_cast<u32x4 *>(dst + k) = w;
+      reinterpret_cast<Loose *>(dst + k)->v = w;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -239,7 +302,6 @@ struct RowSource {
   const void *a, *b, *c;
   float eps;
   void *residual_out;
-  int aligned;                 // a, b, c and residual_out are 16-byte aligned
 };
 
 // g / (1 + exp(-g)) with the hardware's exponential and reciprocal (an ulp each, 2^-17 in all at the steepest: a 64th of
@@ -251,10 +313,10 @@ __device__ __forceinline__ float silu(float g) {
 
 // Eight elements of a 16-bit row from element k on; what lies behind the row is zero.
 template <int dtype>
-__device__ __forceinline__ void row8(const void *row, int k, int K, int aligned, float (&f)[8]) {
+__device__ __forceinline__ void row8(const void *row, int k, int K, float (&f)[8]) {
   const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
-  if (aligned && k + 8 <= K) {
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(p + k);
+  if (k + 8 <= K) {
+    const u32x4 w = load_loose(p + k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = load16<dtype>((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
   } else {
@@ -313,14 +375,14 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
   float rs = 0.0f;
   float norm0[8];                      // the norm weight of the thread's first piece, asked for ahead of the barrier
   if (MODE == kNorm) {
-    row8<dtype>(src.c, min(8 * tid, K - 1), K, src.aligned, norm0);
+    row8<dtype>(src.c, min(8 * tid, K - 1), K, norm0);
     float ss = 0.0f;
     for (int i = tid; i < pieces; i += 64 * WAVES) {
       float f[8];
-      row8<dtype>(src.a, 8 * i, K, src.aligned, f);
+      row8<dtype>(src.a, 8 * i, K, f);
       if (src.b) {
         float g[8];
-        row8<dtype>(src.b, 8 * i, K, src.aligned, g);
+        row8<dtype>(src.b, 8 * i, K, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(f[j] + g[j]);
       }
@@ -328,7 +390,7 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
       xs[i] = r;
       if (blockIdx.x == 0 && src.residual_out) {
         uint16_t *out = reinterpret_cast<uint16_t *>(src.residual_out);
-        if (src.aligned && 8 * i + 8 <= K) *reinterpret_cast<u32x4 *>(out + 8 * i) = r;
+        if (8 * i + 8 <= K) reinterpret_cast<Loose *>(out + 8 * i)->v = r;
         else
           for (int j = 0; j < 8; ++j)
             if (8 * i + j < K) out[8 * i + j] = (uint16_t)(r[j >> 1] >> (16 * (j & 1)));
@@ -356,19 +418,19 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = norm0[j];
       } else {
-        row8<dtype>(src.c, 8 * i, K, src.aligned, w);
+        row8<dtype>(src.c, 8 * i, K, w);
       }
       const u32x4 r = xs[i];           // (the piece this thread wrote itself)
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(w[j] * (load16<dtype>((uint16_t)(r[j >> 1] >> (16 * (j & 1)))) * rs));
     } else if (MODE == kSilu) {
       float g[8], u[8];
-      row8<dtype>(src.a, 8 * i, K, src.aligned, g);
-      row8<dtype>(src.b, 8 * i, K, src.aligned, u);
+      row8<dtype>(src.a, 8 * i, K, g);
+      row8<dtype>(src.b, 8 * i, K, u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = round16<dtype>(round16<dtype>(silu(g[j])) * u[j]);
     } else {
-      row8<dtype>(src.a, 8 * i, K, src.aligned, f);
+      row8<dtype>(src.a, 8 * i, K, f);
     }
     xs[i] = pack8<dtype>(f);
     float s = 0.0f;
@@ -435,30 +497,58 @@ w4_row_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
   }
 }
 
-// Rows of any stride and type -> rows of the weights' type, columns padded with zeros to whole tiles.
+// Eight elements of row m of the activations, from element k on; what lies behind the matrix is zero.
 template <int dtype>
-__global__ void __launch_bounds__(256)
-w4_stage_rows_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_row, int K, int K_padded,
-                     uint16_t *__restrict__ out) {
-  const int k = blockIdx.x * 256 + threadIdx.x;
-  const int64_t m = blockIdx.y;
-  if (k >= K_padded) return;
-  out[m * K_padded + k] = k < K ? bits16<dtype>(rdkv_load_as_float(x, x_dtype, m * x_stride_row + k)) : (uint16_t)0;
+__device__ __forceinline__ u32x4 rows8(const void *x, int x_dtype, int64_t x_stride_row, int64_t m, int M, int k, int K) {
+  if (m >= M) return u32x4{0, 0, 0, 0};
+  if (x_dtype == dtype && k + 8 <= K) return load_loose(reinterpret_cast<const uint16_t *>(x) + m * x_stride_row + k);
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = k + j < K ? rdkv_load_as_float(x, x_dtype, m * x_stride_row + k + j) : 0.0f;
+  return pack8<dtype>(f);
+}
+template <int dtype>
+__device__ __forceinline__ float sum8(u32x4 v) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = v[i];
+    s += load16<dtype>((uint16_t)pair);
+    s += load16<dtype>((uint16_t)(pair >> 16));
+  }
+  return s;
+}
+// The sum over the lanes of a group's pieces (sixteen lanes hold the pieces of a column tile), in each of them.
+template <int GPC>
+__device__ __forceinline__ float sum_pieces(float s) {
+  s += rdkv_dpp_mov<0xB1>(s);                    // pairs, fours, eights, sixteens
+  s += rdkv_dpp_mov<0x4E>(s);
+  if (GPC <= 2) s += rdkv_dpp_mov<0x141>(s);
+  if (GPC == 1) s += rdkv_dpp_mov<0x140>(s);
+  return s;
 }
 
-// Two to sixteen activation rows: a workgroup takes a row tile of the weights (grid.x) and 16 activation rows (grid.y), its
-// wavefronts share the columns.  The rows' operands come straight from global memory (each is read by
-// one wavefront), the sums X from a product with ones (all columns of it are X, where the lanes need it).
-// x rows 16-byte aligned, K_x a multiple of 8 (what lies behind is taken as zero).
+// Rows as rows of the weights' type, zeros behind their ends up to a multiple of eight elements.
+template <int dtype>
+__global__ void __launch_bounds__(256)
+w4_stage_rows_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_row, int K, int K_out, uint16_t *__restrict__ out) {
+  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+  if (k < K_out) out[m * K_out + k] = k < K ? bits16<dtype>(rdkv_load_as_float(x, x_dtype, m * x_stride_row + k)) : (uint16_t)0;
+}
+
+// Few products: a workgroup takes a row tile of the weights (grid.x) and 16 activation rows (grid.y), its wavefronts share
+// the columns.  The rows' operands come straight from global memory (each is read by one wavefront), the sums X from a
+// product with ones (all columns of it are X, where the lanes need it).  The rows start at 16-byte borders, K is a multiple
+// of eight: what lies behind is taken as zero.
 template <int dtype, int GPC, int WAVES, int U>
 __global__ void __launch_bounds__(64 * WAVES)
 w4_few_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, const uint16_t *__restrict__ x,
-              int64_t x_stride_row, const uint16_t *__restrict__ bias, int M, int N, int K_x, int n_tiles_k,
+              int64_t x_stride_row, const uint16_t *__restrict__ bias, int M, int N, int K, int n_tiles_k,
               uint16_t *__restrict__ y, int64_t y_stride_row) {
   __shared__ float s_acc[WAVES][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 4, n = lane & 15;
   const int tn = blockIdx.x, m0 = blockIdx.y * 16;
-  const uint16_t *row = x + (int64_t)min(m0 + n, M - 1) * x_stride_row;
+  const uint16_t *row = x + (int64_t)min(m0 + n, M - 1) * x_stride_row;       // (behind the last one: not stored)
   const u32x4 *tile = codes + (int64_t)tn * n_tiles_k * 64 + lane;
   const uint32_t *words = scales + (int64_t)tn * n_tiles_k * GPC * 16 + n;
   constexpr uint32_t one2 = dtype == RDKV_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
@@ -468,15 +558,15 @@ w4_few_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
   auto load = [&](int k0, Piece &p) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int kc = k0 + u < k_end ? k0 + u : k0;
+      const int kc = min(k0 + u, n_tiles_k - 1);       // (behind the run: loaded, not used)
       p.q[u] = load_stream(tile + (int64_t)kc * 64);
 #pragma unroll
       for (int g = 0; g < GPC; ++g) p.w[u][g] = words[(kc * GPC + g) * 16];
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         const int k = kc * kTileCols + 32 * d + 8 * c;
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + (k < K_x ? k : 0));
-        p.a[u][d] = k < K_x ? v : u32x4{0, 0, 0, 0};
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + (k < K ? k : 0));
+        p.a[u][d] = k < K ? v : u32x4{0, 0, 0, 0};
       }
     }
   };
@@ -516,7 +606,8 @@ w4_few_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
   for (int i = 0; i < 4; ++i) s_acc[wave][(4 * c + i) * 16 + n] = acc[i];
   __syncthreads();
   if (tid < 256) {
-    const int m = m0 + (tid >> 4), r = tn * 16 + (tid & 15);
+    const int m = m0 + (tid >> 4);
+    const int64_t r = (int64_t)tn * 16 + (tid & 15);
     if (m < M && r < N) {
       float s = 0.0f;
 #pragma unroll
@@ -531,63 +622,36 @@ w4_few_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scal
 // columns 8 p .. 8 p + 7, of row m at 16-byte slot 16 p + m: what lane 16 c + m reads for p = 4 d + c), zeros behind the
 // matrix, and forms the sums X; every workgroup of the second launch then copies whole blocks.  Blocks follow each other by
 // column tile within MT tiles of rows: the operands of the MT tiles, then their sums [group][row].
-template <int dtype>
-__device__ __forceinline__ float sum8(u32x4 v) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = v[i];
-    s += load16<dtype>((uint16_t)pair);
-    s += load16<dtype>((uint16_t)(pair >> 16));
-  }
-  return s;
-}
 template <int GPC, int MT>
 struct Block { u32x4 x[MT * 256]; float sum[GPC][16 * MT]; };
 
 template <int dtype, int GPC, int MT>
 __global__ void __launch_bounds__(256)
-w4_blocks_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_row, int aligned, int M, int K,
-                 Block<GPC, MT> *__restrict__ out) {
+w4_blocks_kernel(const void *__restrict__ x, int x_dtype, int64_t x_stride_row, int M, int K, Block<GPC, MT> *__restrict__ out) {
   const int tid = threadIdx.x, piece = tid & 15, m = tid >> 4;
   const int kc = blockIdx.x, mt = blockIdx.y % MT;
-  const int64_t row = (int64_t)blockIdx.y * 16 + m;
   Block<GPC, MT> &block = out[(int64_t)(blockIdx.y / MT) * gridDim.x + kc];
-  const int k = kc * kTileCols + 8 * piece;
-  u32x4 v = {0, 0, 0, 0};
-  if (row < M) {
-    if (aligned && k + 8 <= K) {
-      v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(x) + row * x_stride_row + k);
-    } else {
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = k + j < K ? rdkv_load_as_float(x, x_dtype, row * x_stride_row + k + j) : 0.0f;
-      v = pack8<dtype>(f);
-    }
-  }
+  const u32x4 v = rows8<dtype>(x, x_dtype, x_stride_row, (int64_t)blockIdx.y * 16 + m, M, kc * kTileCols + 8 * piece, K);
   block.x[mt * 256 + piece * 16 + m] = v;
-  float s = sum8<dtype>(v);
-  s += rdkv_dpp_mov<0xB1>(s);                    // lanes of a pair, of four, of eight, of sixteen
-  s += rdkv_dpp_mov<0x4E>(s);
-  if (GPC <= 2) s += rdkv_dpp_mov<0x141>(s);
-  if (GPC == 1) s += rdkv_dpp_mov<0x140>(s);
+  const float s = sum_pieces<GPC>(sum8<dtype>(v));
   if (piece % (16 / GPC) == 0) block.sum[piece / (16 / GPC)][16 * mt + m] = s;
 }
 
-// A workgroup takes 16 MT activation rows by 128 rows of the weights.  Two sets of four wavefronts take the column tiles in
-// turn (even, odd); a set copies the next block to LDS while it computes on the one before.  A wavefront multiplies it
-// with two row tiles of the weights.
-template <int dtype, int GPC, int MT>
+// A workgroup of eight wavefronts takes 16 MT activation rows by NT row tiles of the weights for each wavefront of a set.  SETS
+// sets take the column tiles in turn; a set copies the next block to LDS while it computes on the one before.  Two sets of
+// four wavefronts with two row tiles each (wide: 128 rows of the weights), or, where that leaves compute units without work,
+// four sets of two wavefronts with one (narrow: 32 rows).
+template <int dtype, int GPC, int MT, int NT, int SETS>
 __global__ void __launch_bounds__(512)
 w4_tile_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, const Block<GPC, MT> *__restrict__ blocks,
                const uint16_t *__restrict__ bias, int M, int N, int n_tiles_n, int n_tiles_k, uint16_t *__restrict__ y,
                int64_t y_stride_row) {
-  constexpr int NT = 2, kSums = GPC * 16 * MT;
-  static_assert(kSums <= 256, "a set's threads copy one sum each");
-  __shared__ Block<GPC, MT> s_block[2][2];        // [set][buffer]
-  const int tid = threadIdx.x, lane = tid & 63, set = __builtin_amdgcn_readfirstlane(tid >> 8),
-            wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), c = lane >> 4, n = lane & 15, st = tid & 255;
-  const int tn0 = blockIdx.x * 8 + wave * NT, m0 = blockIdx.y * (16 * MT);
+  constexpr int kWaves = 8 / SETS, kThreads = 64 * kWaves, kCopies = MT * 256 / kThreads, kSums = GPC * 16 * MT,
+                kSumCopies = (kSums + kThreads - 1) / kThreads;
+  __shared__ Block<GPC, MT> s_block[SETS][2];        // [set][buffer]
+  const int tid = threadIdx.x, lane = tid & 63, set = __builtin_amdgcn_readfirstlane(tid / kThreads),
+            wave = __builtin_amdgcn_readfirstlane(tid / 64 % kWaves), c = lane >> 4, n = lane & 15, st = tid % kThreads;
+  const int tn0 = (blockIdx.x * kWaves + wave) * NT, m0 = blockIdx.y * (16 * MT);
   const Block<GPC, MT> *from = blocks + (int64_t)blockIdx.y * n_tiles_k;
   const u32x4 *tile[NT];
   const uint32_t *words[NT];
@@ -603,16 +667,19 @@ w4_tile_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ sca
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   struct Weights { u32x4 q[NT]; uint32_t w[NT][GPC]; };
-  struct Copy { u32x4 x[MT]; float sum; };
+  struct Copy { u32x4 x[kCopies]; float sum[kSumCopies]; };
   auto load_x = [&](int kc, Copy &v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) v.x[j] = from[kc].x[256 * j + st];
-    v.sum = (&from[kc].sum[0][0])[min(st, kSums - 1)];
+    for (int j = 0; j < kCopies; ++j) v.x[j] = from[kc].x[kThreads * j + st];
+#pragma unroll
+    for (int j = 0; j < kSumCopies; ++j) v.sum[j] = (&from[kc].sum[0][0])[min(kThreads * j + st, kSums - 1)];
   };
   auto store_x = [&](Block<GPC, MT> &to, const Copy &v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) to.x[256 * j + st] = v.x[j];
-    if (st < kSums) (&to.sum[0][0])[st] = v.sum;
+    for (int j = 0; j < kCopies; ++j) to.x[kThreads * j + st] = v.x[j];
+#pragma unroll
+    for (int j = 0; j < kSumCopies; ++j)
+      if (kThreads * j + st < kSums) (&to.sum[0][0])[kThreads * j + st] = v.sum[j];
   };
   auto load_w = [&](int kc, Weights &w) __attribute__((always_inline)) {
 #pragma unroll
@@ -657,10 +724,10 @@ w4_tile_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ sca
       }
     }
   };
-  // Both sets make the same number of steps.  The loads of a step are issued two steps ahead (behind the last tile: the
+  // All sets make the same number of steps.  The loads of a step are issued two steps ahead (behind the last tile: the
   // last one again, not used; without a branch, so that a wait leaves the younger loads in flight).
-  const int steps = (n_tiles_k + 1) / 2;
-  auto at = [&](int step) __attribute__((always_inline)) { return min(2 * step + set, n_tiles_k - 1); };
+  const int steps = (n_tiles_k + SETS - 1) / SETS;
+  auto at = [&](int step) __attribute__((always_inline)) { return min(SETS * step + set, n_tiles_k - 1); };
   Weights w[2];
   Copy xv[2];
   load_x(at(0), xv[0]);
@@ -675,35 +742,42 @@ w4_tile_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ sca
       const int step = step0 + j;
       if (step < steps) {
         load_x(at(step + 2), xv[j]);
-        if (2 * step + set < n_tiles_k) compute(s_block[set][j], w[j]);
+        if (SETS * step + set < n_tiles_k) compute(s_block[set][j], w[j]);
         load_w(at(step + 2), w[j]);
         store_x(s_block[set][j ^ 1], xv[j ^ 1]);
         __syncthreads();
       }
     }
   }
-  // the odd set's sums join the even one's (all reads of the blocks are behind the barrier)
-  static_assert(sizeof(s_block) >= 4 * NT * MT * 256 * 4, "the sums of a set fit the blocks");
+  // the other sets' sums join the first one's, in their order (all reads of the blocks are behind the barrier)
+  static_assert(sizeof(s_block) >= (SETS - 1) * kWaves * NT * MT * 256 * 4, "the sums of the sets fit the blocks");
   f32x4 *join = reinterpret_cast<f32x4 *>(&s_block[0][0]) + wave * (NT * MT * 64) + lane;
-  if (set == 1) {
+  constexpr int kJoin = kWaves * NT * MT * 64;       // of a set
+  if (set > 0) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) join[(nt * MT + mt) * 64] = acc[nt][mt];
+      for (int mt = 0; mt < MT; ++mt) join[(set - 1) * kJoin + (nt * MT + mt) * 64] = acc[nt][mt];
   }
   __syncthreads();
-  if (set == 1) return;
+  if (set > 0) return;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int64_t r = (int64_t)(tn0 + nt) * 16 + n;
     const float b = bias && r < N ? load16<dtype>(bias[r]) : 0.0f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const f32x4 other = join[(nt * MT + mt) * 64];
+      f32x4 sum = acc[nt][mt];
+#pragma unroll
+      for (int o = 1; o < SETS; ++o) {
+        const f32x4 other = join[(o - 1) * kJoin + (nt * MT + mt) * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += other[i];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int m = m0 + 16 * mt + 4 * c + i;
-        if (m < M && r < N) y[(int64_t)m * y_stride_row + r] = bits16<dtype>(acc[nt][mt][i] + other[i] + b);
+        if (m < M && r < N) y[(int64_t)m * y_stride_row + r] = bits16<dtype>(sum[i] + b);
       }
     }
   }
@@ -769,7 +843,6 @@ struct Rows {
   const void *x;
   int x_dtype;
   int64_t x_stride;
-  int aligned;                 // rows of the weights' type that can be read in 16-byte pieces
   int K;
   const uint16_t *bias;
   int M, N;
@@ -777,35 +850,48 @@ struct Rows {
   int64_t y_stride;
   void *workspace;
 };
-template <int dtype, int GPC, int MT>
-void launch_tile(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
-  const unsigned blocks = (unsigned)rdkv_cdiv(r.M, 16 * MT);
-  auto *at = reinterpret_cast<Block<GPC, MT> *>(r.workspace);
-  hipLaunchKernelGGL((w4_blocks_kernel<dtype, GPC, MT>), dim3(sh.n_tiles_k, blocks * MT), dim3(256), 0, s, r.x, r.x_dtype, r.x_stride,
-                     r.aligned, r.M, r.K, at);
-  hipLaunchKernelGGL((w4_tile_kernel<dtype, GPC, MT>), dim3((unsigned)rdkv_cdiv(sh.n_tiles_n, 8), blocks), dim3(512), 0, s,
-                     (const u32x4 *)codes, scales, at, r.bias, r.M, r.N, sh.n_tiles_n, sh.n_tiles_k, r.y, r.y_stride);
-}
+// How the rows are multiplied, by the number of workgroups that each form makes; K = 4096, groups of 128, in us:
+//   - up to two tiles of 16 x 16 results for each compute unit: w4_few_kernel, whose one launch keeps nothing in LDS
+//     (few / narrow tiles: 2 x 4096 5.3 / 8.7, 64 x 1024 7.1 / 16.3, 32 x 4096 11.2 / 11.5, but 24 x 6144 14.2 / 11.4);
+//   - beyond, wide tiles of the workgroup where they make work for three quarters of the compute units, of 64 rows if
+//     possible (64 x 28672: wide 64 rows 27.5, wide 32 rows 29.5, narrow 42.8; 64 x 14336: wide 32 rows 18.6, wide 64 rows
+//     25.8, narrow 25.9), narrow ones otherwise (64 x 4096: 11.8 against 17.5 wide, 16 x 16384: 12.2 against 16.6).
+bool few(int M, int N) { return rdkv_cdiv(N, kTileRows) * rdkv_cdiv(M, 16) <= 2 * compute_units(); }
+int64_t few_row(int K) { return rdkv_cdiv(K, 8) * 8; }        // elements of a staged row
+
 template <int dtype, int GPC>
 void launch_few(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
   const uint16_t *x = (const uint16_t *)r.x;
   int64_t stride = r.x_stride;
-  int K_x = r.K;
-  if (!r.aligned) {            // a padded copy first
-    K_x = sh.n_tiles_k * kTileCols;
-    stride = K_x;
+  int K = r.K;
+  if (r.x_dtype != dtype || K % 8 || !aligned16(x) || (r.M > 1 && stride % 8)) {
+    stride = K = (int)few_row(K);
     x = (const uint16_t *)r.workspace;
-    hipLaunchKernelGGL(w4_stage_rows_kernel<dtype>, dim3((unsigned)rdkv_cdiv(K_x, 256), r.M), dim3(256), 0, s, r.x, r.x_dtype, r.x_stride,
-                       r.K, K_x, (uint16_t *)r.workspace);
+    hipLaunchKernelGGL(w4_stage_rows_kernel<dtype>, dim3((unsigned)rdkv_cdiv(K, 256), r.M), dim3(256), 0, s, r.x, r.x_dtype,
+                       r.x_stride, r.K, K, (uint16_t *)r.workspace);
   }
-  hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 16, 2>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(1024), 0, s,
-                     (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K_x, sh.n_tiles_k, r.y, r.y_stride);
+  hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 8, 2>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(512), 0, s,
+                     (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K, sh.n_tiles_k, r.y, r.y_stride);
+}
+template <int dtype, int GPC, int MT, int NT, int SETS>
+void launch_tile(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
+  const unsigned blocks = (unsigned)rdkv_cdiv(r.M, 16 * MT);
+  auto *at = reinterpret_cast<Block<GPC, MT> *>(r.workspace);
+  hipLaunchKernelGGL((w4_blocks_kernel<dtype, GPC, MT>), dim3(sh.n_tiles_k, blocks * MT), dim3(256), 0, s, r.x, r.x_dtype, r.x_stride,
+                     r.M, r.K, at);
+  hipLaunchKernelGGL((w4_tile_kernel<dtype, GPC, MT, NT, SETS>), dim3((unsigned)rdkv_cdiv(sh.n_tiles_n, 8 / SETS * NT), blocks), dim3(512), 0,
+                     s, (const u32x4 *)codes, scales, at, r.bias, r.M, r.N, sh.n_tiles_n, sh.n_tiles_k, r.y, r.y_stride);
 }
 template <int dtype, int GPC>
 void launch_rows(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
-  if (r.M <= 16) launch_few<dtype, GPC>(sh, codes, scales, r, s);
-  else if (r.M <= 32) launch_tile<dtype, GPC, 2>(sh, codes, scales, r, s);
-  else launch_tile<dtype, GPC, 4>(sh, codes, scales, r, s);
+  const int full = compute_units() * 3 / 4;
+  const int64_t across = rdkv_cdiv(sh.n_tiles_n, 8);         // workgroups of the wide form
+  if (few(r.M, r.N)) launch_few<dtype, GPC>(sh, codes, scales, r, s);
+  else if (r.M <= 16 && across >= full) launch_tile<dtype, GPC, 1, 2, 2>(sh, codes, scales, r, s);
+  else if (r.M <= 16) launch_tile<dtype, GPC, 1, 1, 4>(sh, codes, scales, r, s);
+  else if (r.M > 32 && across * rdkv_cdiv(r.M, 64) >= full) launch_tile<dtype, GPC, 4, 2, 2>(sh, codes, scales, r, s);
+  else if (across * rdkv_cdiv(r.M, 32) >= full) launch_tile<dtype, GPC, 2, 2, 2>(sh, codes, scales, r, s);
+  else launch_tile<dtype, GPC, 2, 1, 4>(sh, codes, scales, r, s);
 }
 
 }  // namespace
@@ -827,11 +913,10 @@ RDKV_API int rdkv_w4_quantize(const void *W, int64_t w_stride_row, int N, int K,
   if (rc != RDKV_OK || N == 0) return rc;
   RDKV_REQUIRE(W && codes && scales && aligned16(codes), "%s: null or misaligned pointer", fn);
   RDKV_REQUIRE(w_stride_row >= K || N == 1, "%s: rows overlap (stride %lld, K=%d)", fn, (long long)w_stride_row, K);
-  const int aligned = aligned16(W) && w_stride_row % 8 == 0;
   const dim3 grid((unsigned)rdkv_cdiv(sh.n_tiles, 4));
 #define RDKV_W4_QUANTIZE(DT, GPC)                                                                                     \
   hipLaunchKernelGGL((w4_quantize_kernel<DT, GPC>), grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t *)W,      \
-                     w_stride_row, N, K, aligned, (int64_t)sh.n_tiles_k, sh.n_tiles, (u32x4 *)codes, scales)
+                     w_stride_row, N, K, (uint32_t)sh.n_tiles_k, (uint32_t)sh.n_tiles, (u32x4 *)codes, scales)
 #define RDKV_W4_QUANTIZE_ANY(DT)                         \
   do {                                                   \
     if (sh.gpc == 1) RDKV_W4_QUANTIZE(DT, 1);            \
@@ -858,7 +943,7 @@ RDKV_API int rdkv_w4_pack(const uint8_t *q, int64_t q_stride_row, const void *sc
   const dim3 grid((unsigned)rdkv_cdiv(sh.n_tiles, 4));
 #define RDKV_W4_PACK(GPC)                                                                                            \
   hipLaunchKernelGGL((w4_pack_kernel<GPC>), grid, dim3(256), 0, (hipStream_t)stream, q, q_stride_row, scale, scale_dtype, \
-                     scale_stride_row, zero, zero_stride_row, N, K, (int64_t)sh.n_tiles_k, sh.n_tiles, (u32x4 *)codes, scales)
+                     scale_stride_row, zero, zero_stride_row, N, K, (uint32_t)sh.n_tiles_k, (uint32_t)sh.n_tiles, (u32x4 *)codes, scales)
   if (sh.gpc == 1) RDKV_W4_PACK(1);
   else if (sh.gpc == 2) RDKV_W4_PACK(2);
   else RDKV_W4_PACK(4);
@@ -875,11 +960,10 @@ RDKV_API int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, i
   if (rc != RDKV_OK || N == 0) return rc;
   RDKV_REQUIRE(codes && scales && out && aligned16(codes), "%s: null or misaligned pointer", fn);
   RDKV_REQUIRE(out_stride_row >= K || N == 1, "%s: output rows overlap", fn);
-  const int aligned = aligned16(out) && out_stride_row % 8 == 0;
   const dim3 grid((unsigned)rdkv_cdiv(sh.n_tiles, 4));
 #define RDKV_W4_DEQUANT(DT, GPC)                                                                                       \
   hipLaunchKernelGGL((w4_dequant_kernel<DT, GPC>), grid, dim3(256), 0, (hipStream_t)stream, (const u32x4 *)codes, scales, \
-                     N, K, aligned, (int64_t)sh.n_tiles_k, sh.n_tiles, (uint16_t *)out, out_stride_row)
+                     N, K, (uint32_t)sh.n_tiles_k, (uint32_t)sh.n_tiles, (uint16_t *)out, out_stride_row)
 #define RDKV_W4_DEQUANT_ANY(DT)                       \
   do {                                                \
     if (sh.gpc == 1) RDKV_W4_DEQUANT(DT, 1);          \
@@ -894,12 +978,12 @@ RDKV_API int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, i
   return RDKV_OK;
 }
 
-RDKV_API int64_t rdkv_w4_linear_workspace_bytes(int M, int K) {
-  if (M <= 0 || K <= 0) return 0;
-  const int64_t n_tiles_k = rdkv_cdiv(K, kTileCols);
-  if (M <= 16) return M * n_tiles_k * kTileCols * 2;
-  // whole blocks of 32 or 64 rows, their sums at the finest groups
-  return rdkv_cdiv(M, M <= 32 ? 32 : 64) * n_tiles_k * (int64_t)(M <= 32 ? sizeof(Block<4, 2>) : sizeof(Block<4, 4>));
+RDKV_API int64_t rdkv_w4_linear_workspace_bytes(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || (M == 1 && K <= kRowMaxK)) return 0;
+  if (few(M, N)) return M * few_row(K) * 2;
+  // whole blocks of 16, 32 or 64 rows, their sums at the finest groups
+  const int64_t block = M <= 16 ? sizeof(Block<4, 1>) : M <= 32 ? sizeof(Block<4, 2>) : sizeof(Block<4, 4>);
+  return rdkv_cdiv(M, M <= 16 ? 16 : M <= 32 ? 32 : 64) * rdkv_cdiv(K, kTileCols) * block;
 }
 
 RDKV_API int rdkv_w4_linear(const void *codes, const uint32_t *scales, const void *x, int x_dtype, int64_t x_stride_row,
@@ -909,28 +993,25 @@ RDKV_API int rdkv_w4_linear(const void *codes, const uint32_t *scales, const voi
   Shape sh;
   const int rc = check_shape(fn, N, K, group, dtype, &sh);
   if (rc != RDKV_OK) return rc;
-  RDKV_REQUIRE(M >= 0 && M <= 1 << 20, "%s: %d rows", fn, M);
+  RDKV_REQUIRE(M >= 0 && M <= 1 << 19, "%s: %d rows", fn, M);
   if (N == 0 || M == 0) return RDKV_OK;
   RDKV_REQUIRE(codes && scales && x && y && aligned16(codes), "%s: null or misaligned pointer", fn);
   RDKV_REQUIRE(x_dtype == dtype || x_dtype == RDKV_DTYPE_F32, "%s: x must have the weights' type or be fp32", fn);
   RDKV_REQUIRE(M == 1 || (x_stride_row >= 0 && y_stride_row >= N), "%s: output rows overlap", fn);
   hipStream_t s = (hipStream_t)stream;
   if (M == 1 && K <= kRowMaxK) {
-    const RowSource src = {x, nullptr, nullptr, 0.0f, nullptr, aligned16(x)};
+    const RowSource src = {x, nullptr, nullptr, 0.0f, nullptr};
     if (x_dtype == RDKV_DTYPE_F32) launch_row_any<kFromF32>(dtype, sh, codes, scales, src, bias, N, K, y, s);
     else launch_row_any<kPlain>(dtype, sh, codes, scales, src, bias, N, K, y, s);
     RDKV_CHECK_LAUNCH(fn);
     return RDKV_OK;
   }
-  const int aligned = x_dtype == dtype && aligned16(x) && (M == 1 || x_stride_row % 8 == 0) && K % 8 == 0;
-  if (M > 16 || !aligned) {
-    const int64_t need = rdkv_w4_linear_workspace_bytes(M, K);
-    if (!workspace || workspace_bytes < need || !aligned16(workspace)) {
-      rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
-      return RDKV_EWORKSPACE;
-    }
+  const int64_t need = rdkv_w4_linear_workspace_bytes(M, N, K);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+    rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
+    return RDKV_EWORKSPACE;
   }
-  const Rows r = {x, x_dtype, x_stride_row, aligned, K, (const uint16_t *)bias, M, N, (uint16_t *)y, y_stride_row, workspace};
+  const Rows r = {x, x_dtype, x_stride_row, K, (const uint16_t *)bias, M, N, (uint16_t *)y, y_stride_row, workspace};
 #define RDKV_W4_ROWS(DT)                                              \
   do {                                                                \
     if (sh.gpc == 1) launch_rows<DT, 1>(sh, codes, scales, r, s);     \
@@ -955,8 +1036,7 @@ RDKV_API int rdkv_w4_linear_norm(const void *codes, const uint32_t *scales, cons
   RDKV_REQUIRE(codes && scales && x && norm_weight && y && aligned16(codes), "%s: null or misaligned pointer", fn);
   RDKV_REQUIRE(!residual_out || (residual_out != x && residual_out != delta),
                "%s: residual_out must not alias the inputs (every workgroup reads them)", fn);
-  const RowSource src = {x, delta, norm_weight, eps, residual_out,
-                         aligned16(x) && aligned16(delta) && aligned16(norm_weight) && aligned16(residual_out)};
+  const RowSource src = {x, delta, norm_weight, eps, residual_out};
   launch_row_any<kNorm>(dtype, sh, codes, scales, src, bias, N, K, y, (hipStream_t)stream);
   RDKV_CHECK_LAUNCH(fn);
   return RDKV_OK;
@@ -970,7 +1050,7 @@ RDKV_API int rdkv_w4_linear_silu(const void *codes, const uint32_t *scales, cons
   if (rc != RDKV_OK || N == 0) return rc;
   RDKV_REQUIRE(K <= kRowMaxK, "%s: K=%d exceeds %d", fn, K, kRowMaxK);
   RDKV_REQUIRE(codes && scales && gate && up && y && aligned16(codes), "%s: null or misaligned pointer", fn);
-  const RowSource src = {gate, up, nullptr, 0.0f, nullptr, aligned16(gate) && aligned16(up)};
+  const RowSource src = {gate, up, nullptr, 0.0f, nullptr};
   launch_row_any<kSilu>(dtype, sh, codes, scales, src, bias, N, K, y, (hipStream_t)stream);
   RDKV_CHECK_LAUNCH(fn);
   return RDKV_OK;

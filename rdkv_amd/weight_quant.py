@@ -159,7 +159,7 @@ def linear(x: torch.Tensor, q: QuantizedWeight, bias: Optional[torch.Tensor] = N
         return out
     lib = _lib.load()
     with torch.cuda.device(dev):
-        need = 0 if M == 1 and q.K <= _MAX_ROW_K else lib.rdkv_w4_linear_workspace_bytes(M, q.K)
+        need = lib.rdkv_w4_linear_workspace_bytes(M, q.N, q.K)
         # (the call's own, so that graphs that hold such calls may replay side by side)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.rdkv_w4_linear(q.codes.data_ptr(), q.scales.data_ptr(), rows.data_ptr(), _lib.DTYPE_CODE[x.dtype],

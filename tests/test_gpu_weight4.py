@@ -66,6 +66,29 @@ def test_quantizer_codes_scales_and_values(N, K, G, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("G", [32, 128])
+def test_quantizer_codes_of_quotients_between_two_codes(dtype, G):
+    """Quotients in the middle of two whole numbers and a hair off it, at small and large scales: the codes are those of the
+    correctly rounded division, rounded to even.  A row's range is 15 units, some with another width in the last bits."""
+    require_gpu()
+    g = torch.Generator().manual_seed(G)
+    N, K = 1024, 512
+    unit = 2.0 ** torch.randint(-13, 12, (N, 1), generator=g).double()
+    if dtype == BF16:
+        unit[: N // 2] = 2.0 ** torch.randint(-122, 122, (N // 2, 1), generator=g).double()
+    w = torch.randint(-16, 17, (N, K), generator=g).double() / 2
+    w[:, ::G], w[:, 1::G] = -7.5, 7.5
+    w[1::2] *= 1 + torch.randint(-3, 4, (N // 2, K), generator=g) * torch.finfo(dtype).eps
+    w[2::4, 1::G] *= 1 + torch.randint(0, 9, (N // 4, 1), generator=g) * torch.finfo(dtype).eps
+    w = (w * unit).to(dtype)
+    codes, s, z = _quantize_ref(w, G)
+    q = wq.quantize_weight(w.to(DEV), G)
+    exp = _packed(codes.to(torch.uint8), s, z.to(torch.uint8), G, dtype)
+    assert torch.equal(q.scales, exp.scales) and torch.equal(q.codes, exp.codes)
+
+
+@pytest.mark.gpu
 def test_quantizer_of_values_that_are_no_numbers_and_of_tiny_ones():
     require_gpu()
     w = torch.randn(20, 256, generator=torch.Generator().manual_seed(3)).to(BF16)
@@ -122,6 +145,30 @@ def test_products_of_whole_numbers_are_exact(N, K, G, dtype):
         wide = torch.full((M, K + 3), float("nan"), dtype=dtype)
         wide[:, 1:K + 1] = x                     # rows of another stride that start off a 16-byte border
         assert torch.equal(wq.linear(wide.to(DEV)[:, 1:K + 1], q, bias.to(DEV)).cpu(), exp), f"{M} strided rows"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(5, 8209, 264), (16, 24600, 136), (17, 4113, 700), (33, 2100, 1000), (20, 24600, 130),
+                                   (40, 24600, 300), (1030, 1500, 260), (2, 8200, 8), (9, 24577, 127)])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_larger_products_of_whole_numbers_are_exact(M, N, K, G, dtype):
+    """As above, where one to sixty-four rows share a tile of the weights and tiles end inside the matrix."""
+    require_gpu()
+    codes, scale, zero = _integers(N, K, G, M + N)
+    W = _dense64(codes, scale, zero, G).to(DEV)
+    q = _packed(codes, scale, zero, G, dtype)
+    g = torch.Generator().manual_seed(M)
+    x = torch.randint(-2, 3, (M, K), generator=g).to(dtype).to(DEV)
+    bias = torch.randint(-8, 9, (N,), generator=g).to(dtype).to(DEV)
+    exp = x.double() @ W.t()
+    guard = torch.full((M * N + 4096,), 7.0, dtype=dtype, device=DEV)
+    assert torch.equal(wq.linear(x, q), exp.to(dtype))
+    assert torch.equal(wq.linear(x.float(), q, bias), (exp + bias.double()).to(dtype))
+    wide = torch.full((M, K + 3), float("nan"), dtype=dtype, device=DEV)
+    wide[:, 1:K + 1] = x
+    assert torch.equal(wq.linear(wide[:, 1:K + 1], q, out=guard[:M * N].view(M, N)), exp.to(dtype))
+    assert bool((guard[M * N:] == 7).all())
 
 
 @pytest.mark.gpu
@@ -270,9 +317,10 @@ def test_refusals_of_the_c_interface():
     for bad in (dict(G=48), dict(G=0), dict(dt=0), dict(xd=2), dict(K=0), dict(N=-1), dict(M=-1), dict(codes=None),
                 dict(scales=None), dict(x=None), dict(y=None), dict(codes=one + 8), dict(ys=15), dict(M=2_000_000)):
         assert linear(**bad) == _lib.RDKV_EINVAL, bad
-    for bad in (dict(xd=0), dict(x=one + 2), dict(xs=65), dict(K=63), dict(M=1, K=40000, xd=0),
-                dict(xd=0, ws=one, wb=511), dict(xd=0, ws=one + 8, wb=512)):
-        assert linear(**bad) == _lib.RDKV_EWORKSPACE, bad
+    need = lib.rdkv_w4_linear_workspace_bytes
+    for bad in (dict(M=17, xd=0), dict(M=1, K=40000, xd=0), dict(M=2, K=7), dict(M=2, N=8208, ys=8208), dict(ws=one, wb=255),
+                dict(M=1000, N=800, ys=800, ws=one, wb=need(1000, 800, 64) - 1), dict(M=17, xd=0, ws=one + 8, wb=1 << 20)):
+        assert linear(**{**bad, "xs": 1 << 16}) == _lib.RDKV_EWORKSPACE, bad
     assert linear(M=0) == _lib.RDKV_OK and linear(N=0) == _lib.RDKV_OK
     assert lib.rdkv_w4_linear_norm(one, one, one, one, one, 0.0, one, None, 16, 64, 32, 1, one, None) == _lib.RDKV_EINVAL
     assert b"alias" in lib.rdkv_last_error()
@@ -284,7 +332,10 @@ def test_refusals_of_the_c_interface():
     assert lib.rdkv_w4_dequant(one, one, 2, 64, 32, 1, one, 63, None) == _lib.RDKV_EINVAL
     assert lib.rdkv_w4_codes_bytes(17, 129) == 4 * 1024 and lib.rdkv_w4_scale_words(17, 129, 32) == 4 * 64
     assert lib.rdkv_w4_codes_bytes(-1, 5) == 0 and lib.rdkv_w4_scale_words(5, 5, 5) == 0
-    assert lib.rdkv_w4_linear_workspace_bytes(3, 129) == 3 * 512
+    assert need(0, 9, 64) == need(9, 0, 64) == need(1, 9, 32768) == 0 and need(1, 16, 32769) == 32776 * 2
+    assert need(2, 16, 7) == 2 * 8 * 2 and need(16, 8192, 129) == 16 * 136 * 2
+    assert need(16, 8208, 8192) == 64 * (4096 + 256) and need(17, 8192, 129) == 2 * (8192 + 512)
+    assert need(65, 8192, 128) == 2 * (16384 + 1024)
 
 
 def test_no_cpu_path():
