@@ -268,9 +268,11 @@ __device__ __forceinline__ u32x4 operand(uint32_t w) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) b[r] = (w >> (4 * r)) & 0x000f000fu;
   } else {
-    b[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
+    uint32_t fields = 0x00780078u;
+    asm("" : "+v"(fields));              // (in a vector register: one instruction takes the mask and the exponent)
+    b[0] = ((w << 3) & fields) | 0x41804180u;
 #pragma unroll
-    for (int r = 1; r < 4; ++r) b[r] = ((w >> (4 * r - 3)) & 0x00780078u) | 0x41804180u;
+    for (int r = 1; r < 4; ++r) b[r] = ((w >> (4 * r - 3)) & fields) | 0x41804180u;
   }
   return b;
 }
