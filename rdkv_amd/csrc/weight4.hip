@@ -44,6 +44,10 @@ template <int dtype>
 __device__ __forceinline__ float load16(uint16_t bits) {
   return dtype == RDKV_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, bits) : __uint_as_float((uint32_t)bits << 16);
 }
+template <int dtype>
+__device__ __forceinline__ uint16_t bits16(float v) {
+  return dtype == RDKV_DTYPE_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : rdkv_float_to_bf16_bits(v);
+}
 __device__ __forceinline__ uint32_t scale_word(float s, uint32_t zero) {
   // 20 significant bits, rounded half up in magnitude; an infinity stays one, a NaN a NaN
   const uint32_t bits = __float_as_uint(s);
@@ -230,30 +234,41 @@ __global__ void __launch_bounds__(256)
 w4_dequant_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ scales, int N, int K,
                   uint32_t n_tiles_k, uint32_t n_tiles, uint16_t *__restrict__ out, int64_t out_stride_row) {
   const TileAt t = tile_at(n_tiles_k);
-  if (t.tile >= n_tiles || t.row >= N) return;
-  const u32x4 q = codes[t.tile * 64 + t.lane];
-  uint16_t *dst = out + t.row * out_stride_row;
+  if (t.tile >= n_tiles) return;
+  // The pieces p of the rows r change lanes through LDS, at slot 16 r + (p ^ r) of the wavefront's own, so that sixteen lanes
+  // write a row's 256 bytes (28672 x 4096 bf16: 51 us, 5.8 TB/s; 82 with 64 bytes of sixteen rows at a time).
+  __shared__ u32x4 s_tile[4][256];
+  u32x4 *mine = s_tile[threadIdx.x >> 6];
+  const int n = t.lane & 15;
+  const u32x4 q = load_stream(codes + t.tile * 64 + t.lane);
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
-    const uint32_t word = scales[(t.tile * GPC + d * GPC / 4) * 16 + (t.lane & 15)];
+    const uint32_t word = scales[(t.tile * GPC + d * GPC / 4) * 16 + n];
     const float s = word_scale(word), z = (float)word_zero(word);
-    const int k = t.col0 + 32 * d + 8 * t.c;
-    uint16_t h[8];
+    u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 4; ++i) {
       // (a 5-bit integer times 20 bits: exact in fp32, rounded once to the type)
-      const float v = ((float)((q[d] >> field_shift(j)) & 15u) - z) * s;
-      h[j] = dtype == RDKV_DTYPE_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : rdkv_float_to_bf16_bits(v);
+      const float lo = ((float)((q[d] >> (4 * i)) & 15u) - z) * s, hi = ((float)((q[d] >> (4 * i + 16)) & 15u) - z) * s;
+      w[i] = bits16<dtype>(lo) | (uint32_t)bits16<dtype>(hi) << 16;
     }
-    if (k + 8 <= K) {
-      u32x4 w;
+    mine[16 * n + ((4 * d + t.c) ^ n)] = w;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-      reinterpret_cast<Loose *>(dst + k)->v = w;
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * i + t.c, k = t.col0 + 8 * n;
+    const int64_t row = t.row - n + r;
+    const u32x4 w = mine[16 * r + (n ^ r)];
+    if (row >= N) continue;
+    uint16_t *dst = out + row * out_stride_row + k;
+    if (k + 8 <= K) {
+      reinterpret_cast<Loose *>(dst)->v = w;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (k + j < K) dst[k + j] = h[j];
+        if (k + j < K) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
     }
   }
 }
@@ -292,10 +307,6 @@ __device__ __forceinline__ float add_group(uint32_t w, float D, float X, float a
 template <int dtype>
 __device__ __forceinline__ float round16(float v) {
   return dtype == RDKV_DTYPE_F16 ? (float)(_Float16)v : __uint_as_float((uint32_t)rdkv_float_to_bf16_bits(v) << 16);
-}
-template <int dtype>
-__device__ __forceinline__ uint16_t bits16(float v) {
-  return dtype == RDKV_DTYPE_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : rdkv_float_to_bf16_bits(v);
 }
 
 // How one activation row reaches LDS, as in gemv.hip.
