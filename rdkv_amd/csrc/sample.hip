@@ -783,12 +783,13 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
 // shows in the counters' sum; the patterns are then counted again with 32 bits, half of them at a time.
 struct Values {                          // LDS
   uint32_t words[1 << 15];               // counter of key k: word_of(k), its half k / 2^15 (or all of it, of one half)
+  uint32_t aside[1024];
   uint64_t part_mass[4][16];
   uint32_t part_count[4][16];
   double table[kPerOctave];
   uint64_t least, base_mass, upto;
   uint32_t total, base_count, place, seg_count[18];
-  int max_key, group, key, seg_first[18], index;
+  int max_key, skipped, group, key, seg_first[18], index;
 };
 // Neighbouring keys lie in neighbouring banks, and so do keys 32 apart (a thread reads 16 neighbours).
 __device__ __forceinline__ uint32_t word_of(uint32_t key) { return (key & 0x7fffu) ^ ((key >> 5) & 31u); }
@@ -819,21 +820,27 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
 #pragma unroll
     for (int i = 0; i < (1 << 13) / 1024; ++i) words[i * 1024 + tid] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    auto one = [&](uint32_t key) __attribute__((always_inline)) {        // (the upper half is not looked at)
+    // Masked tokens share one value: a value that a quarter of a wavefront's lanes start with is counted aside, in a word of
+    // the lane's own, and left out if it is no number or fills half of the row (rows of 128256 with 99 % masked: 31 us; 250 with
+    // their counts added up at one address, beyond the 16 bits of a counter).  Any key will do.
+    uint32_t aside = 0;
+    bool some = false;
+    s.aside[tid] = 0;
+    auto one = [&](uint32_t key, bool look_aside) __attribute__((always_inline)) {        // (the upper half is not looked at)
       const uint32_t upper = (key >> 15) & 1;
-      if (half < 0) atomicAdd(&s.words[word_of(key)], upper * 0xffffu + 1u);
-      else if ((int)upper == half) atomicAdd(&s.words[word_of(key)], 1u);
+      const bool common = look_aside && (uint16_t)key == (uint16_t)aside;
+      uint32_t *at = common ? &s.aside[tid] : &s.words[word_of(key)];
+      if (half < 0) atomicAdd(at, !common && upper ? 0x10000u : 1u);
+      else if (common || (int)upper == half) atomicAdd(at, 1u);
     };
-    auto two = [&](uint32_t bits) __attribute__((always_inline)) {
+    auto keys_of = [&](uint32_t bits) __attribute__((always_inline)) {
       if (half >= 0) {                                                  // (-0 counts as 0)
         if ((bits & 0xffffu) == 0x8000u) bits &= 0xffff0000u;
         if ((bits >> 16) == 0x8000u) bits &= 0xffffu;
       }
       typedef short short2_t __attribute__((ext_vector_type(2)));
       const uint32_t negative = __builtin_bit_cast(uint32_t, __builtin_bit_cast(short2_t, bits) >> (short)15);
-      const uint32_t keys = bits ^ (negative | 0x80008000u);
-      one(keys);
-      one(keys >> 16);
+      return bits ^ (negative | 0x80008000u);
     };
     for (int i0 = 0; i0 < row.pieces; i0 += U * 1024) {
       u32x4 v[U];
@@ -842,22 +849,51 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
         const int i = i0 + k * 1024 + tid;
         v[k] = row.piece(i < row.pieces ? i : 0);
       }
+      if (i0 == 0) {
+        const uint32_t pair = v[0][0], first = keys_of(pair) & 0xffffu;
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i0 + k * 1024 + tid < row.pieces) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t pair = v[k][e];
-            two(pair);
+        for (int of = 0; of < 64; of += 16) {
+          const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)first, of);
+          if (__popcll(__ballot(first == key)) >= 16) {
+            aside = key;
+            some = true;
           }
         }
       }
+      auto all = [&](bool look_aside) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (i0 + k * 1024 + tid < row.pieces) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t pair = v[k][e], keys = keys_of(pair);
+              one(keys, look_aside);
+              one(keys >> 16, look_aside);
+            }
+          }
+        }
+      };
+      if (some) all(true);
+      else all(false);
     }
     const int tail = row.head + row.pieces * 8, n_ends = row.head + vocab - tail;
     if (tid < n_ends) {
       uint32_t bits = reinterpret_cast<const uint16_t *>(row.p)[tid < row.head ? tid : tail + tid - row.head];
       if (half >= 0 && bits == 0x8000u) bits = 0;
-      one(bits ^ (0x8000u | ((bits >> 15) * 0x7fffu)));
+      one(bits ^ (0x8000u | ((bits >> 15) * 0x7fffu)), true);
+    }
+    const uint32_t n = wave_total(s.aside[tid]);                        // (the lane's own word, after its own additions)
+    if (lane == 63 && n) {
+      const uint32_t upper = aside >> 15;
+      const bool counts = allowed((int)aside);
+      if (half < 0 && (!counts || n >= 4096)) {      // (sixteen of them might not fit a counter)
+        atomicAdd(&s.total, n);
+        if (counts) atomicMax(&s.skipped, (int)aside);
+      } else if (half < 0) {
+        atomicAdd(&s.words[word_of(aside)], n << (16 * upper));
+      } else if ((int)upper == half) {
+        atomicAdd(&s.words[word_of(aside)], n);
+      }
     }
     __syncthreads();
   };
@@ -870,7 +906,7 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   if (tid == 0) {
     s.least = 0;
     s.total = 0;
-    s.max_key = -1;
+    s.max_key = s.skipped = -1;
   }
   count(-1);
   if (tid == 0) {          // -0 joins 0, its neighbour
@@ -880,7 +916,7 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       zero += c << 16;
       minus -= c;
     } else {
-      s.total = 1;         // (the sum will not be the row's length)
+      s.total += 1;        // (the sum will not be the row's length)
     }
   }
   __syncthreads();
@@ -956,7 +992,10 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   };
   const bool greedy = !(set.T > 0.0f);
   look();
-  const bool wide = s.total != (uint32_t)vocab;
+  bool wide = s.total != (uint32_t)vocab;
+  const int skipped = s.skipped;         // the largest value that was left out: it has to have no weight
+  if (skipped >= 0)
+    wide |= max_key <= skipped || (!greedy && bins_below(scale_of(value(max_key), set.T, top), value(skipped)) < (double)kBins);
   if (wide) {
     __syncthreads();
     if (tid == 0) s.max_key = -1;

@@ -162,6 +162,37 @@ def test_masks_infinities_and_no_numbers(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("V", [131, 9000, 70_001, 140_000])
+def test_rows_that_one_value_fills(V, dtype):
+    """One value at most places, as a mask leaves it or as the largest of all: it has to count where it has weight (the
+    temperature is high, it is the largest, nothing else is left) and in top-k, and may not where it has none."""
+    require_gpu()
+    g = torch.Generator().manual_seed(V)
+    low, inf = torch.finfo(dtype).min, float("inf")
+    x = torch.randn(16, V, generator=g)
+    fill = torch.rand(16, V, generator=g) < 0.98
+    for row, v in enumerate([-inf, low, -1e4, float("nan"), -8.0, 3.0, 9.0, 0.0, -0.0]):
+        x[row, fill[row]] = v
+    x[9] = torch.where(fill[9], low, -inf)                     # nothing else is left
+    x[10] = torch.where(fill[10], torch.tensor(-inf), torch.tensor(low))
+    x[11, : V // 2] = low                                      # some wavefronts' value, and another's
+    x[11, V // 2:] = -inf
+    x[11, V // 3] = 1.0
+    x[12] = low
+    x[12, V - 1] = x[12, 0] = low / 2
+    x[13, fill[13]] = torch.finfo(dtype).max
+    x[14] = torch.where(fill[14], 0.0, x[14])
+    x[14, ::2] = torch.where(x[14, ::2] == 0, -0.0, x[14, ::2])
+    x[15, V // 5:] = low
+    u = torch.rand(16, generator=g).numpy()
+    big = float(torch.finfo(dtype).max) / 4
+    for setting in (dict(), dict(T=0.0), dict(k=40), dict(k=V // 2, T=2.0), dict(p=0.9, min_p=0.05), dict(T=big), dict(k=V - 3, p=0.7, T=big),
+                    _mixed(16, V, V)):
+        check(x.to(dtype), u, **setting, what=str(setting))
+
+
+@pytest.mark.gpu
 def test_borders_and_ties():
     """Borders that are exact in any arithmetic: equal weights, a share that falls on a token's end."""
     require_gpu()
