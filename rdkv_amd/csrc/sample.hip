@@ -10,10 +10,11 @@
 // so that a sum does not depend on the order, the launch's shape or the atomics that form it, and a border between two
 // tokens lies where 64 bits put it.
 //
-// Three launches.  Maximum: the slices of a row leave their largest logit.  Histogram: sums (and, under top-k,
-// counts) of the weights in bins of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup
-// per row adds the bins up, which tells in which bins the searches can end, collects those bins' tokens in one pass over the
-// row and resolves the searches among them, by further bins over (logit, index) while they are many.
+// Many rows of 16-bit logits: one launch that counts the bit patterns, further below.  fp32, or a few rows: three launches.
+// Maximum: the slices of a row leave their largest logit.  Histogram: sums (and, under top-k, counts) of the weights in bins
+// of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup per row adds the bins up, which
+// tells in which bins the searches can end, collects those bins' tokens in one pass over the row and resolves the searches
+// among them, by further bins over (logit, index) while they are many.
 #include "rdkv_common.h"
 #include "rope_device.h"
 
@@ -1205,50 +1206,57 @@ int weight_bits(int vocab) {             // of the largest weight: all of them t
 }
 
 // Slices of a row: about four workgroups per compute unit over the rows, none of less than 256 pieces.
-int slices_of(int rows, int vocab) {
-  const int pieces = vocab / 4;
+int slices_of(int rows, int vocab, int elements) {
+  const int pieces = vocab / elements;
   const int want = (int)rdkv_cdiv(1024, rows), most = (int)rdkv_cdiv(pieces, 256);
   int s = want < most ? want : most;
   s = s < kMaxSlices ? s : kMaxSlices;
   return s < 1 ? 1 : s;
 }
 
-int launch_slices(const char *fn, const float *logits, int64_t stride, int rows, int vocab, const Settings &set,
+template <int dtype>
+int launch_slices(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set,
                   const float *uniform, int64_t *token, float *logprob, const Advance &adv, RowSpace *space,
                   hipStream_t s) {
-  constexpr int F32 = RDKV_DTYPE_F32;
-  const int slices = slices_of(rows, vocab), top = weight_bits(vocab);
+  const int slices = slices_of(rows, vocab, Row<dtype>::EPP), top = weight_bits(vocab);
   for (int r = 0; r < rows; r += 65535) {                  // (a grid's second dimension)
     const int n = rows - r < 65535 ? rows - r : 65535;
-    const float *from = logits + (int64_t)r * stride;
+    const void *from = reinterpret_cast<const char *>(logits) + (int64_t)r * stride * (dtype == RDKV_DTYPE_F32 ? 4 : 2);
     Settings part = set;
     if (part.temperature) part.temperature += r;
     if (part.top_k) part.top_k += r;
     if (part.top_p) part.top_p += r;
     if (part.min_p) part.min_p += r;
-    hipLaunchKernelGGL(sample_max_kernel<F32>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
+    hipLaunchKernelGGL(sample_max_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
     RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_bins_kernel<F32>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
+    hipLaunchKernelGGL(sample_bins_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
     RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_choose_kernel<F32>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
+    hipLaunchKernelGGL(sample_choose_kernel<dtype>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
                        uniform + r, space + r, token + r, logprob ? logprob + r : nullptr, adv);
     RDKV_CHECK_LAUNCH(fn);
   }
   return RDKV_OK;
 }
+// A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, fp16, without masks and
+// with 99 % masked: 128256 logits, 1 row 26.8 / 34.0 and 22.0 / 31.2, 8 rows 29.7 / 36.0 and 24.5 / 33.3, 16 rows 38.0 / 36.1 and
+// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 4000 logits, 1 row 18.8 / 20.3 and 18.9 / 16.6.
+bool by_slices(int rows, int dtype) { return dtype == RDKV_DTYPE_F32 || rows <= 12; }
+
 int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, int dtype, const Settings &set,
                   const float *uniform, int64_t *token, float *logprob, const Advance &adv, void *workspace,
                   hipStream_t s) {
-  if (dtype == RDKV_DTYPE_F32)
-    return launch_slices(fn, reinterpret_cast<const float *>(logits), stride, rows, vocab, set, uniform, token, logprob, adv,
-                         reinterpret_cast<RowSpace *>(workspace), s);
-  const int top = weight_bits(vocab);
-  if (dtype == RDKV_DTYPE_F16)
-    hipLaunchKernelGGL(sample_values_kernel<RDKV_DTYPE_F16>, dim3(rows), dim3(1024), sizeof(Values), s, logits, stride, vocab, top, set,
-                       uniform, token, logprob, adv);
-  else
-    hipLaunchKernelGGL(sample_values_kernel<RDKV_DTYPE_BF16>, dim3(rows), dim3(1024), sizeof(Values), s, logits, stride, vocab, top, set,
-                       uniform, token, logprob, adv);
+  auto *space = reinterpret_cast<RowSpace *>(workspace);
+#define RDKV_SAMPLE(DT)                                                                                                       \
+  do {                                                                                                                        \
+    if (by_slices(rows, DT)) return launch_slices<DT>(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, space, s); \
+    if (DT != RDKV_DTYPE_F32)                                                                                                 \
+      hipLaunchKernelGGL(sample_values_kernel<DT == RDKV_DTYPE_F32 ? RDKV_DTYPE_F16 : DT>, dim3(rows), dim3(1024), sizeof(Values), s, \
+                         logits, stride, vocab, weight_bits(vocab), set, uniform, token, logprob, adv);                       \
+  } while (0)
+  if (dtype == RDKV_DTYPE_F32) RDKV_SAMPLE(RDKV_DTYPE_F32);
+  else if (dtype == RDKV_DTYPE_F16) RDKV_SAMPLE(RDKV_DTYPE_F16);
+  else RDKV_SAMPLE(RDKV_DTYPE_BF16);
+#undef RDKV_SAMPLE
   RDKV_CHECK_LAUNCH(fn);
   return RDKV_OK;
 }
@@ -1275,7 +1283,7 @@ int sample(const char *fn, const void *logits, int64_t stride, int rows, int voc
 }  // namespace
 
 RDKV_API int64_t rdkv_sample_workspace_bytes(int rows, int dtype) {
-  return rows <= 0 || dtype != RDKV_DTYPE_F32 ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace);
+  return rows <= 0 || !by_slices(rows, dtype) ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace);
 }
 
 RDKV_API int rdkv_sample_rows(const void *logits, int64_t stride_row, int rows, int vocab, int dtype,

@@ -41,10 +41,18 @@ def oracle(logits, u, T, k, p, min_p):
 def check(logits, u, T=1.0, k=0, p=1.0, min_p=0.0, what=""):
     """Runs the rows, with settings per row or shared, and compares; returns the tokens."""
     B = logits.shape[0]
-    dev = lambda v, t: torch.as_tensor(v, dtype=t).to(DEV) if np.ndim(v) else v  # noqa: E731
-    token, logprob = sampling.sample_tokens(logits.to(DEV), torch.as_tensor(u, dtype=F32).to(DEV), temperature=dev(T, F32),
-                                            top_k=dev(k, torch.int32), top_p=dev(p, F32), min_p=dev(min_p, F32))
+
+    def run(rows):
+        dev = lambda v, t: torch.as_tensor(v, dtype=t)[rows].to(DEV) if np.ndim(v) else v  # noqa: E731
+        return sampling.sample_tokens(logits.to(DEV)[rows.to(DEV)], torch.as_tensor(u, dtype=F32)[rows].to(DEV), temperature=dev(T, F32),
+                                      top_k=dev(k, torch.int32), top_p=dev(p, F32), min_p=dev(min_p, F32))
+
+    token, logprob = run(torch.arange(B))
     assert token.dtype == torch.int64 and logprob.dtype == F32
+    # a few rows and many go different ways: the rows repeated to twenty, and the last ones alone
+    for rows in (torch.arange(20) % B, torch.arange(max(0, B - 4), B)):
+        again, lp = run(rows)
+        assert torch.equal(again, token[rows.to(DEV)]) and torch.equal(lp, logprob[rows.to(DEV)]), f"{what} rows {rows.tolist()}"
     f32 = lambda v: np.broadcast_to(np.asarray(v, np.float32).astype(np.float64), (B,))  # noqa: E731
     T, p, min_p, u = f32(T), f32(p), f32(min_p), f32(u)
     k = np.broadcast_to(k, (B,))
@@ -351,7 +359,8 @@ def test_refusals_of_the_c_interface():
     one = 1 << 20                    # a pointer that is looked at, never followed
     s = _lib.RdkvSampling(temperature_value=1.0, top_p_value=1.0)
     need = lib.rdkv_sample_workspace_bytes(2, 0)
-    assert need > 0 and lib.rdkv_sample_workspace_bytes(0, 0) == lib.rdkv_sample_workspace_bytes(-3, 0) == lib.rdkv_sample_workspace_bytes(2, 1) == 0
+    assert need > 0 and lib.rdkv_sample_workspace_bytes(0, 0) == lib.rdkv_sample_workspace_bytes(-3, 0) == lib.rdkv_sample_workspace_bytes(13, 1) == 0
+    assert lib.rdkv_sample_workspace_bytes(2, 1) == lib.rdkv_sample_workspace_bytes(2, 2) == need
 
     def rows(logits=one, stride=64, n=2, vocab=64, dt=0, u=one, settings=ctypes.addressof(s), token=one, ws=one, nb=need):
         return lib.rdkv_sample_rows(logits, stride, n, vocab, dt, u, settings, token, None, ws, nb, None)
