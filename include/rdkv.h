@@ -392,7 +392,7 @@ int rdkv_w4_pack(const uint8_t *q, int64_t q_stride_row, const void *scale, int 
 int rdkv_w4_dequant(const void *codes, const uint32_t *scales, int N, int K, int group, int dtype, void *out,
                     int64_t out_stride_row, void *stream);
 /* y[m, n] = sum_k x[m, k] * W[n, k] (+ bias[n]): x [M, K] of x_dtype = `dtype`, or fp32 (rounded to `dtype` first), y [M, N]
- * and bias [N] of `dtype`; fp32 accumulation in a fixed order.  M up to 2^19, any N, K.  The
+ * (it overlaps none of the inputs) and bias [N] of `dtype`; fp32 accumulation in a fixed order.  M up to 2^19, any N, K.  The
  * workspace (rdkv_w4_linear_workspace_bytes on the device of the call, 16-byte aligned; 0 for one row of up to 32768
  * elements) takes the rows in the order that the products read them in. */
 int64_t rdkv_w4_linear_workspace_bytes(int M, int N, int K);

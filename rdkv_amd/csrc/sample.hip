@@ -1214,10 +1214,15 @@ int slices_of(int rows, int vocab, int elements) {
   return s < 1 ? 1 : s;
 }
 
+// A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, fp16, without masks and
+// with 99 % masked: 128256 logits, 1 row 26.8 / 34.0 and 22.0 / 31.2, 8 rows 29.7 / 36.0 and 24.5 / 33.3, 16 rows 38.0 / 36.1 and
+// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 4000 logits, 1 row 18.8 / 20.3 and 18.9 / 16.6.
+bool by_slices(int rows, int dtype) { return dtype == RDKV_DTYPE_F32 || rows <= 12; }
+
 template <int dtype>
-int launch_slices(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set,
-                  const float *uniform, int64_t *token, float *logprob, const Advance &adv, RowSpace *space,
-                  hipStream_t s) {
+int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set, const float *uniform,
+                  int64_t *token, float *logprob, const Advance &adv, RowSpace *space, hipStream_t s) {
+  const bool slices_first = by_slices(rows, dtype);
   const int slices = slices_of(rows, vocab, Row<dtype>::EPP), top = weight_bits(vocab);
   for (int r = 0; r < rows; r += 65535) {                  // (a grid's second dimension)
     const int n = rows - r < 65535 ? rows - r : 65535;
@@ -1227,37 +1232,20 @@ int launch_slices(const char *fn, const void *logits, int64_t stride, int rows, 
     if (part.top_k) part.top_k += r;
     if (part.top_p) part.top_p += r;
     if (part.min_p) part.min_p += r;
-    hipLaunchKernelGGL(sample_max_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
-    RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_bins_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
-    RDKV_CHECK_LAUNCH(fn);
-    hipLaunchKernelGGL(sample_choose_kernel<dtype>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
-                       uniform + r, space + r, token + r, logprob ? logprob + r : nullptr, adv);
+    float *lp = logprob ? logprob + r : nullptr;
+    if (slices_first) {
+      hipLaunchKernelGGL(sample_max_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
+      RDKV_CHECK_LAUNCH(fn);
+      hipLaunchKernelGGL(sample_bins_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
+      RDKV_CHECK_LAUNCH(fn);
+      hipLaunchKernelGGL(sample_choose_kernel<dtype>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
+                         uniform + r, space + r, token + r, lp, adv);
+    } else if constexpr (dtype != RDKV_DTYPE_F32) {
+      hipLaunchKernelGGL(sample_values_kernel<dtype>, dim3(n), dim3(1024), sizeof(Values), s, from, stride, vocab, top, part, uniform + r,
+                         token + r, lp, adv);
+    }
     RDKV_CHECK_LAUNCH(fn);
   }
-  return RDKV_OK;
-}
-// A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, fp16, without masks and
-// with 99 % masked: 128256 logits, 1 row 26.8 / 34.0 and 22.0 / 31.2, 8 rows 29.7 / 36.0 and 24.5 / 33.3, 16 rows 38.0 / 36.1 and
-// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 4000 logits, 1 row 18.8 / 20.3 and 18.9 / 16.6.
-bool by_slices(int rows, int dtype) { return dtype == RDKV_DTYPE_F32 || rows <= 12; }
-
-int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, int dtype, const Settings &set,
-                  const float *uniform, int64_t *token, float *logprob, const Advance &adv, void *workspace,
-                  hipStream_t s) {
-  auto *space = reinterpret_cast<RowSpace *>(workspace);
-#define RDKV_SAMPLE(DT)                                                                                                       \
-  do {                                                                                                                        \
-    if (by_slices(rows, DT)) return launch_slices<DT>(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, space, s); \
-    if (DT != RDKV_DTYPE_F32)                                                                                                 \
-      hipLaunchKernelGGL(sample_values_kernel<DT == RDKV_DTYPE_F32 ? RDKV_DTYPE_F16 : DT>, dim3(rows), dim3(1024), sizeof(Values), s, \
-                         logits, stride, vocab, weight_bits(vocab), set, uniform, token, logprob, adv);                       \
-  } while (0)
-  if (dtype == RDKV_DTYPE_F32) RDKV_SAMPLE(RDKV_DTYPE_F32);
-  else if (dtype == RDKV_DTYPE_F16) RDKV_SAMPLE(RDKV_DTYPE_F16);
-  else RDKV_SAMPLE(RDKV_DTYPE_BF16);
-#undef RDKV_SAMPLE
-  RDKV_CHECK_LAUNCH(fn);
   return RDKV_OK;
 }
 
@@ -1277,7 +1265,10 @@ int sample(const char *fn, const void *logits, int64_t stride, int rows, int voc
   }
   const Settings set = {sampling->temperature, sampling->top_k, sampling->top_p, sampling->min_p,
                         sampling->temperature_value, sampling->top_k_value, sampling->top_p_value, sampling->min_p_value};
-  return launch_sample(fn, logits, stride, rows, vocab, dtype, set, uniform, token, logprob, adv, workspace, (hipStream_t)stream);
+  auto *launch = dtype == RDKV_DTYPE_F32 ? launch_sample<RDKV_DTYPE_F32>
+                 : dtype == RDKV_DTYPE_F16 ? launch_sample<RDKV_DTYPE_F16> : launch_sample<RDKV_DTYPE_BF16>;
+  return launch(fn, logits, stride, rows, vocab, set, uniform, token, logprob, adv, reinterpret_cast<RowSpace *>(workspace),
+                (hipStream_t)stream);
 }
 
 }  // namespace

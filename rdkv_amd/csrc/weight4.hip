@@ -65,7 +65,7 @@ __device__ __forceinline__ TileAt tile_at(uint32_t n_tiles_k) {
   TileAt t;
   t.lane = threadIdx.x & 63;
   t.c = t.lane >> 4;
-  const uint32_t tile = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // below 2^31 + 3
+  const uint32_t tile = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // below 2^26
   t.tile = tile;
   t.row = (int64_t)(tile / n_tiles_k) * kTileRows + (t.lane & 15);
   t.col0 = (int)(tile % n_tiles_k * kTileCols);        // (below K, which is at most 2^31 - 256)
@@ -822,7 +822,8 @@ int check_shape(const char *fn, int N, int K, int group, int dtype, Shape *s) {
   s->n_tiles_k = (int)rdkv_cdiv(K, kTileCols);
   s->gpc = kTileCols / group;
   s->n_tiles = (int64_t)s->n_tiles_n * s->n_tiles_k;
-  RDKV_REQUIRE(s->n_tiles <= (int64_t)0x7fffffff, "%s: a matrix of %d x %d is too large", fn, N, K);
+  // (four tiles to 256 threads, below 2^32 of them: 1.4e11 weights)
+  RDKV_REQUIRE(s->n_tiles < (int64_t)1 << 26, "%s: a matrix of %d x %d is too large", fn, N, K);
   return RDKV_OK;
 }
 

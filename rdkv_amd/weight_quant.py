@@ -134,6 +134,13 @@ def _check_bias(q: QuantizedWeight, bias: Optional[torch.Tensor]) -> Optional[to
     return bias.contiguous()
 
 
+def _overlap(out: torch.Tensor, t: Optional[torch.Tensor]) -> bool:
+    if t is None or t.numel() == 0 or out.numel() == 0:
+        return False
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    return t.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < t.data_ptr() + last * t.element_size()
+
+
 def linear(x: torch.Tensor, q: QuantizedWeight, bias: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``F.linear(x.to(q.dtype), W, bias)`` for ``x`` [..., K] of ``q.dtype`` or fp32 (rounded to it),
@@ -155,6 +162,7 @@ def linear(x: torch.Tensor, q: QuantizedWeight, bias: Optional[torch.Tensor] = N
         out = torch.empty(x.shape[:-1] + (q.N,), dtype=q.dtype, device=dev)
     assert tuple(out.shape) == tuple(x.shape[:-1]) + (q.N,) and out.dtype == q.dtype and out.is_contiguous(), \
         "out: contiguous rows of the weights' type"
+    assert not _overlap(out, rows) and not _overlap(out, bias), "out must not overlap the inputs (every workgroup reads them)"
     if M == 0 or q.N == 0:
         return out
     lib = _lib.load()

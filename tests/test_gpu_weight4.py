@@ -245,6 +245,12 @@ def test_empty_and_odd_calls():
     assert torch.equal(wq.linear(one, q).cpu(), exp[0, :1].expand(5, 20))
     out = torch.empty(2, 3, 20, dtype=F16, device=DEV)
     assert wq.linear(x.to(DEV), q, out=out) is out and torch.equal(out.cpu(), exp)
+    square = wq.quantize_weight(torch.eye(64, dtype=F16, device=DEV), 32)
+    both = torch.zeros(20, 64, dtype=F16, device=DEV)
+    for y in (both[:10], both[5:15]):                                # (whole rows of one buffer, and rows in part)
+        with pytest.raises(AssertionError, match="overlap"):
+            wq.linear(both[:10], square, out=y)
+    assert bool((wq.linear(both[:10], square, out=both[10:]) == 0).all())
     none = wq.quantize_weight(torch.zeros(0, 64, dtype=F16, device=DEV), 32)
     assert wq.linear(x.to(DEV), none).shape == (2, 3, 0) and wq.dequantize_weight(none).shape == (0, 64)
 
@@ -315,7 +321,7 @@ def test_refusals_of_the_c_interface():
                                   a["G"], a["dt"], a["y"], a["ys"], a["ws"], a["wb"], None)
 
     for bad in (dict(G=48), dict(G=0), dict(dt=0), dict(xd=2), dict(K=0), dict(N=-1), dict(M=-1), dict(codes=None),
-                dict(scales=None), dict(x=None), dict(y=None), dict(codes=one + 8), dict(ys=15), dict(M=2_000_000)):
+                dict(scales=None), dict(x=None), dict(y=None), dict(codes=one + 8), dict(ys=15), dict(M=2_000_000), dict(N=1 << 20, ys=1 << 20, K=1 << 17)):
         assert linear(**bad) == _lib.RDKV_EINVAL, bad
     need = lib.rdkv_w4_linear_workspace_bytes
     for bad in (dict(M=17, xd=0), dict(M=1, K=40000, xd=0), dict(M=2, K=7), dict(M=2, N=8208, ys=8208), dict(ws=one, wb=255),
