@@ -884,8 +884,18 @@ void launch_few(const Shape &sh, const void *codes, const uint32_t *scales, cons
     hipLaunchKernelGGL(w4_stage_rows_kernel<dtype>, dim3((unsigned)rdkv_cdiv(K, 256), r.M), dim3(256), 0, s, r.x, r.x_dtype,
                        r.x_stride, r.K, K, (uint16_t *)r.workspace);
   }
-  hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 8, 2>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(512), 0, s,
-                     (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K, sh.n_tiles_k, r.y, r.y_stride);
+  // Wavefronts that share the columns, tiles a step: 8 and 2 for one to eight tiles a wavefront (5 x 6144 x 4096 7.8 us, 8.7 with
+  // 8 and 1, 9.1 with 16 and 1); one tile each at most, and a second would be loaded for nothing: 12 x 1024 x 1024 3.6 against 4.4; beyond
+  // K = 8192, 16 and 1: 8 x 4096 x 14336 13.8 against 15.4.
+  if (sh.n_tiles_k <= 8)
+    hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 8, 1>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(512), 0, s,
+                       (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K, sh.n_tiles_k, r.y, r.y_stride);
+  else if (sh.n_tiles_k <= 64)
+    hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 8, 2>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(512), 0, s,
+                       (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K, sh.n_tiles_k, r.y, r.y_stride);
+  else
+    hipLaunchKernelGGL((w4_few_kernel<dtype, GPC, 16, 1>), dim3(sh.n_tiles_n, (unsigned)rdkv_cdiv(r.M, 16)), dim3(1024), 0, s,
+                       (const u32x4 *)codes, scales, x, stride, r.bias, r.M, r.N, K, sh.n_tiles_k, r.y, r.y_stride);
 }
 template <int dtype, int GPC, int MT, int NT, int SETS>
 void launch_tile(const Shape &sh, const void *codes, const uint32_t *scales, const Rows &r, hipStream_t s) {
