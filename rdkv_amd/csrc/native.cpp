@@ -33,6 +33,7 @@ namespace {
   X(rdkv_decode_fused) X(rdkv_decode_fused_zone_c) X(rdkv_decode_fused_workspace_bytes)                           \
   X(rdkv_unpack_layer) X(rdkv_stream_plan_layer) X(rdkv_pack_layer) X(rdkv_plan_layers)                                                           \
   X(rdkv_select_layer_start) X(rdkv_pack_layers_stream)                                                          \
+  X(rdkv_w4_quantize) X(rdkv_w4_dequant) X(rdkv_w4_codes_bytes) X(rdkv_w4_scale_words)                           \
   X(rdkv_w4_linear) X(rdkv_w4_linear_workspace_bytes) X(rdkv_w4_linear_norm) X(rdkv_w4_linear_silu)              \
   X(rdkv_sample_rows) X(rdkv_sample_workspace_bytes)
 struct Library {
@@ -779,6 +780,48 @@ struct Quantized {
   }
 };
 
+// weight, group, stream -> codes, scales
+PyObject *w4_quantize(PyObject *const *a, Py_ssize_t) {
+  const at::Tensor &w = tensor(a[0]);
+  const int64_t group = whole(a[1]);
+  void *stream = address(a[2]);
+  const int code = dtype_code(w);
+  plain(w.is_cuda() && w.dim() == 2 && (code == RDKV_DTYPE_F16 || code == RDKV_DTYPE_BF16));
+  const int64_t N = w.size(0), K = w.size(1);
+  plain(N >= 1 && K >= 1 && N <= 0x7ffffff0 && K <= 0x7fffff00 && w.stride(1) == 1 && (N == 1 || w.stride(0) >= K));
+  plain(group == 32 || group == 64 || group == 128);
+  at::Tensor codes, scales;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(w.device());
+    const auto dev = at::TensorOptions().device(w.device());
+    codes = at::empty({lib.rdkv_w4_codes_bytes((int)N, (int)K)}, dev.dtype(at::kByte));
+    scales = at::empty({lib.rdkv_w4_scale_words((int)N, (int)K, (int)group)}, dev.dtype(at::kInt));
+    rc = lib.rdkv_w4_quantize(w.data_ptr(), w.stride(0), (int)N, (int)K, (int)group, code, codes.data_ptr(),
+                              reinterpret_cast<uint32_t *>(scales.data_ptr()), stream);
+  }
+  status(rc);
+  Ref c(wrap(codes)), s(wrap(scales));
+  return Ref(PyTuple_Pack(2, c.o, s.o)).release();
+}
+
+// codes, scales, N, K, group, type, stream
+PyObject *w4_dequantize(PyObject *const *a, Py_ssize_t) {
+  const Quantized q(a, 0);
+  void *stream = address(a[6]);
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked u;
+    const c10::DeviceGuard guard(q.codes.device());
+    out = at::empty({q.N, q.K}, q.options(q.codes));
+    rc = lib.rdkv_w4_dequant(q.codes.data_ptr(), q.words(), q.N, q.K, q.group, q.dtype, out.data_ptr(), q.K, stream);
+  }
+  status(rc);
+  return wrap(out);
+}
+
 // x, codes, scales, N, K, group, type, bias or None, stream
 PyObject *w4_linear(PyObject *const *a, Py_ssize_t) {
   const at::Tensor &x = tensor(a[0]);
@@ -937,6 +980,8 @@ PyMethodDef kMethods[] = {
     ENTRY(stream_pack, 12, "The blobs of the layers, or None."),
     ENTRY(decode_attn, 16, "(out, lse) of a decode step, or None."),
     ENTRY(dense_layer, 7, "Dense (K, V) of a packed layer, with its additive mask where one is given; or None."),
+    ENTRY(w4_quantize, 3, "(codes, scale words) of a matrix, or None."),
+    ENTRY(w4_dequantize, 7, "The matrix that codes and scale words stand for, or None."),
     ENTRY(w4_linear, 9, "The product of activation rows with a 4-bit matrix, or None."),
     ENTRY(w4_norm_linear, 12, "(product, residual row) of one row with its norm, or None."),
     ENTRY(w4_silu_linear, 10, "The product of one row with its activation, or None."),

@@ -61,6 +61,12 @@ def quantize_weight(weight: torch.Tensor, group_size: int = 128) -> QuantizedWei
     """Round-to-nearest quantization of ``weight`` [N, K] (fp16 / bf16; rows of any stride) by groups
     of ``group_size`` columns, the last of a row may be short.  The range of a group takes in
     zero, so zeros stay zeros.  A group that holds a NaN or an infinity becomes NaN."""
+    if weight.is_cuda:
+        if _lib.native is None:
+            _lib.load()
+        pair = _lib.native.w4_quantize(weight, group_size, _lib.stream_of(weight.device))
+        if pair is not None:
+            return QuantizedWeight(*pair, *weight.shape, group_size, weight.dtype)
     dev = _lib.require_device(weight)
     assert weight.dim() == 2, f"a matrix, got {tuple(weight.shape)}"
     if weight.stride(1) != 1 or (weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]):
@@ -101,6 +107,10 @@ def pack_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.T
 
 def dequantize_weight(q: QuantizedWeight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The matrix [N, K] that the codes stand for, each value rounded to ``q.dtype``."""
+    if out is None:
+        w = _native("w4_dequantize", q, *_fields(q))
+        if w is not None:
+            return w
     dev = _lib.require_device(q.codes, q.scales, out)
     if out is None:
         out = torch.empty(q.N, q.K, dtype=q.dtype, device=dev)

@@ -297,14 +297,23 @@ def test_plain_calls_take_the_native_way(monkeypatch):
     y = wq.linear(x, q, bias)
     n, r = wq.norm_linear(h, delta, norm, 1e-5, q, bias)
     s = wq.silu_linear(h, up, q)
-    assert calls.taken == ["w4_linear", "w4_norm_linear", "w4_silu_linear"]
+    dense = wq.dequantize_weight(q)
+    again = wq.quantize_weight(dense, 64)
+    assert calls.taken == ["w4_linear", "w4_norm_linear", "w4_silu_linear", "w4_dequantize", "w4_quantize"]
+    del calls.taken[3:], calls.asked[3:]
+    for view in (dense.t().contiguous().t(), torch.cat([dense[:1], dense])[1:]):       # columns of another stride; rows as they are
+        other = wq.quantize_weight(view, 64)
+        assert torch.equal(other.codes, again.codes) and torch.equal(other.scales, again.scales) and other.shape == (50, 300)
+    assert calls.taken[3:] == ["w4_quantize"] and calls.asked[3:] == ["w4_quantize"] * 2
+    del calls.taken[3:], calls.asked[3:]
     general = wq.linear(x.transpose(0, 1), q, bias)                   # rows that are no plain view
     assert calls.taken[3:] == [] and calls.asked[3:] == ["w4_linear"] and torch.equal(general, y.transpose(0, 1))
     wide = torch.stack([bias, bias], 1)[:, 0]                         # a bias of another stride
     assert torch.equal(wq.linear(x, q, wide), y) and torch.equal(wq.norm_linear(h, delta, norm, 1e-5, q, wide)[0], n)
     assert torch.equal(wq.silu_linear(h, up, q, torch.zeros_like(wide)), s) and len(calls.taken) == 4
     monkeypatch.setattr(_lib, "native", type("None_", (), {"__getattr__": lambda self, name: lambda *a: None})())
-    assert torch.equal(wq.linear(x, q, bias), y)
+    assert torch.equal(wq.linear(x, q, bias), y) and torch.equal(wq.dequantize_weight(q), dense)
+    assert torch.equal(wq.quantize_weight(dense, 64).codes, again.codes)
     n2, r2 = wq.norm_linear(h, delta, norm, 1e-5, q, bias)
     assert torch.equal(n2, n) and torch.equal(r2, r) and torch.equal(wq.silu_linear(h, up, q), s)
 
