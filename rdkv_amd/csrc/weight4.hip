@@ -72,6 +72,15 @@ __device__ __forceinline__ TileAt tile_at(uint32_t n_tiles_k) {
   return t;
 }
 
+// The largest of the four lanes 16 c + n that hold a row's pieces, in each of them.
+__device__ __forceinline__ float max_of_row(float v) {
+  typedef unsigned uint2_t __attribute__((ext_vector_type(2)));
+  uint2_t both = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+  both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
 // Eight elements without the first n, zeros behind the others.
 __device__ __forceinline__ u32x4 drop_front(u32x4 v, int n) {
   if (n <= 0) return v;
@@ -143,20 +152,18 @@ w4_quantize_kernel(const uint16_t *__restrict__ W, int64_t w_stride_row, int N, 
         size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2, pair));
       }
     }
-    bool bad = size[0] >= kInfinite || size[1] >= kInfinite;
-#pragma unroll
-    for (int o = 16; o < 64; o <<= 1) {   // the four lanes that share the row
-      lo = fminf(lo, __shfl_xor(lo, o, 64));
-      hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-      bad |= (bool)__shfl_xor((int)bad, o, 64);
-    }
-    float s = word_scale(scale_word((hi - lo) / 15.0f, 0));
-    if (!(s < INFINITY) || bad) s = __builtin_nanf("");
+    if (size[0] >= kInfinite || size[1] >= kInfinite) hi = INFINITY;
+    hi = max_of_row(hi);
+    lo = -max_of_row(-lo);
+    // (hi - lo) / 15 and 1 / s by their remainders too: the first correctly rounded, the second within an ulp
+    const float range = hi - lo, part = range * (1.0f / 15.0f);
+    float s = word_scale(scale_word(__builtin_fmaf(__builtin_fmaf(-part, 15.0f, range), 1.0f / 15.0f, part), 0));
+    if (!(s < INFINITY)) s = __builtin_nanf("");
     if (s < kSmallestScale) s = 1.0f;
     // Correctly rounded quotients without a division for each: q = v * (1 / s) is within a few ulp, its remainder v - q s is
     // exact, and q + (v - q s) (1 / s) before its rounding is within 2^-22 ulp of v / s, which, s having 20 bits, stays
     // 2^-21 ulp away from the middle of two fp32 numbers.  (Not where the remainder could be subnormal.)
-    const float inv = 1.0f / s;
+    const float about = __builtin_amdgcn_rcpf(s), inv = __builtin_fmaf(__builtin_fmaf(-s, about, 1.0f), about, about);
     auto quotient = [&](float w) __attribute__((always_inline)) {
       const float q = w * inv;
       return __builtin_fmaf(__builtin_fmaf(-q, s, w), inv, q);
@@ -173,7 +180,7 @@ w4_quantize_kernel(const uint16_t *__restrict__ W, int64_t w_stride_row, int N, 
     for (int d = g * DPG; d < (g + 1) * DPG; ++d) {
       uint32_t w = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w += __float_as_uint(fminf(fmaxf(quotient(weight(d, j)) + kWhole, from), to)) << field_shift(j);
+      for (int j = 0; j < 8; ++j) w += __float_as_uint(__builtin_amdgcn_fmed3f(quotient(weight(d, j)) + kWhole, from, to)) << field_shift(j);
       out[d] = w - beside;
     }
     if (tiny) {
