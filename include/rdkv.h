@@ -428,7 +428,7 @@ typedef struct RdkvSampling {
   float top_p_value;
   float min_p_value;
 } RdkvSampling;
-int64_t rdkv_sample_workspace_bytes(int rows, int dtype);      /* of a call with so many rows; 0 for 13 or more of fp16 / bf16 */
+int64_t rdkv_sample_workspace_bytes(int rows, int vocab, int dtype);      /* of a call of this size; 0: none is needed */
 /* logits [rows, vocab] of `dtype` (any row stride, vocab at most 2^24), uniform [rows], token [rows], logprob [rows] or NULL. */
 int rdkv_sample_rows(const void *logits, int64_t stride_row, int rows, int vocab, int dtype, const float *uniform,
                      const RdkvSampling *sampling, int64_t *token, float *logprob, void *workspace,

@@ -125,7 +125,7 @@ SIGNATURES = {
     "rdkv_w4_linear": (I, [P, P, P, I, L, P, I, I, I, I, I, P, L, P, L, P]),
     "rdkv_w4_linear_norm": (I, [P, P, P, P, P, F, P, P, I, I, I, I, P, P]),
     "rdkv_w4_linear_silu": (I, [P, P, P, P, P, I, I, I, I, P, P]),
-    "rdkv_sample_workspace_bytes": (L, [I, I]),
+    "rdkv_sample_workspace_bytes": (L, [I, I, I]),
     "rdkv_sample_rows": (I, [P, L, I, I, I, P, P, P, P, P, L, P]),
     "rdkv_sample_advance": (I, [P, I, I, P, I, P, P, P, P, P, P, I, P, ctypes.c_uint32, P, L, P]),
     "rdkv_decode_fused_merge": (I, [P, I, I, I, P, L, P, P, L, P]),

@@ -940,7 +940,7 @@ PyObject *sample_rows(PyObject *const *a, Py_ssize_t) {
     const c10::DeviceGuard guard(logits.device());
     const auto dev = at::TensorOptions().device(logits.device());
     token = at::empty(shape, dev.dtype(at::kLong)), logprob = at::empty(shape, dev.dtype(at::kFloat));
-    const int64_t need = lib.rdkv_sample_workspace_bytes(rows, code);
+    const int64_t need = lib.rdkv_sample_workspace_bytes((int)rows, (int)vocab, code);
     if (need) ws = at::empty({need}, dev.dtype(at::kByte));
     rc = lib.rdkv_sample_rows(logits.data_ptr(), stride, rows, vocab, code, uniform.data_ptr<float>(), &s, token.data_ptr<int64_t>(),
                               logprob.data_ptr<float>(), data(ws), need, stream);

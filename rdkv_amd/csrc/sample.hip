@@ -10,11 +10,11 @@
 // so that a sum does not depend on the order, the launch's shape or the atomics that form it, and a border between two
 // tokens lies where 64 bits put it.
 //
-// Many rows of 16-bit logits: one launch that counts the bit patterns, further below.  fp32, or a few rows: three launches.
-// Maximum: the slices of a row leave their largest logit.  Histogram: sums (and, under top-k, counts) of the weights in bins
-// of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup per row adds the bins up, which
-// tells in which bins the searches can end, collects those bins' tokens in one pass over the row and resolves the searches
-// among them, by further bins over (logit, index) while they are many.
+// Many long rows of 16-bit logits: one launch that counts the bit patterns, further below.  Otherwise three steps, of long
+// rows a launch each.  Maximum: the slices of a row leave their largest logit.  Histogram: sums (and, under top-k, counts) of
+// the weights in bins of 1/32 octave below the maximum; 46 octaves down the weights are 0.  Choice: one workgroup per row adds
+// the bins up, which tells in which bins the searches can end, collects those bins' tokens in one pass over the row and
+// resolves the searches among them, by further bins over (logit, index) while they are many.
 #include "rdkv_common.h"
 #include "rope_device.h"
 
@@ -183,6 +183,29 @@ __device__ __forceinline__ float row_best(const RowSpace &sp, int slices) {
   return rdkv_wave_max(lane < slices ? sp.best[lane] : -INFINITY);
 }
 
+// What a row's bins take in: w >= min_p as bins below the maximum; without top-p nobody asks about what lies beyond.
+struct BinRule {
+  bool counts, least;
+  double least_t, need;
+  __device__ __forceinline__ explicit BinRule(const RowSettings &set) {
+    counts = set.top_k > 0, least = set.min_p > 0.0f;
+    least_t = least ? -log2((double)fminf(set.min_p, 1.0f)) * kPerOctave : 0.0;
+    need = least && !(set.top_p < 1.0f) ? fmin(least_t + 1.0, (double)kBins) : (double)kBins;
+  }
+  __device__ __forceinline__ void add(const Scale &sc, const double *table, uint64_t *mass, uint32_t *count, uint64_t &least_mass,
+                                      float l, bool there) const {
+    double t = bins_below(sc, l);
+    if (t < (there ? need : -INFINITY)) {
+      t = placed(t);
+      const uint64_t w = weight(sc, table, t);
+      const int bin = (int)t;
+      atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)w);
+      if (counts) atomicAdd(&count[bin], 1u);
+      if (least && t <= least_t) least_mass += w;
+    }
+  }
+};
+
 template <int dtype>
 __global__ void __launch_bounds__(256)
 sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, Settings settings,
@@ -196,7 +219,7 @@ sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, i
   const float best = row_best(sp, slices);
   const RowSettings set = row_settings(settings, blockIdx.y);
   if (best == -INFINITY || !(set.T > 0.0f)) return;      // nothing allowed, or the largest is the choice
-  const bool counts = set.top_k > 0, least = set.min_p > 0.0f;
+  const BinRule rule(set);
   fill_table(s_table);
   for (int i = tid; i < kBins; i += 256) {
     s_mass[i] = 0;
@@ -205,28 +228,17 @@ sample_bins_kernel(const void *__restrict__ logits, int64_t stride, int vocab, i
   if (tid == 0) s_least = 0;
   __syncthreads();
   const Scale sc = scale_of(best, set.T, top);
-  // w >= min_p as bins below the maximum; without top-p nobody asks about what lies beyond
-  const double least_t = least ? -log2((double)fminf(set.min_p, 1.0f)) * kPerOctave : 0.0;
-  const double need = least && !(set.top_p < 1.0f) ? fmin(least_t + 1.0, (double)kBins) : (double)kBins;
   const Row<dtype> row(logits, stride, blockIdx.y, vocab);
   const int per = (row.pieces + slices - 1) / slices, begin = min(slice * per, row.pieces), end = min(begin + per, row.pieces);
   uint64_t least_mass = 0;
-  row.template each<256>(begin, end, slice == 0, [&](float l, int i, bool there) __attribute__((always_inline)) {
-    double t = bins_below(sc, l);
-    if (t < (there ? need : -INFINITY)) {
-      t = placed(t);
-      const uint64_t w = weight(sc, s_table, t);
-      const int bin = (int)t;
-      atomicAdd((unsigned long long *)&s_mass[bin], (unsigned long long)w);
-      if (counts) atomicAdd(&s_count[bin], 1u);
-      if (least && t <= least_t) least_mass += w;
-    }
+  row.template each<256>(begin, end, slice == 0, [&](float l, int, bool there) __attribute__((always_inline)) {
+    rule.add(sc, s_table, s_mass, s_count, least_mass, l, there);
   });
-  if (least && least_mass) atomicAdd((unsigned long long *)&s_least, (unsigned long long)least_mass);
+  if (least_mass) atomicAdd((unsigned long long *)&s_least, (unsigned long long)least_mass);
   __syncthreads();
   for (int i = tid; i < kBins; i += 256) {
     if (s_mass[i]) atomicAdd((unsigned long long *)&sp.mass[i], (unsigned long long)s_mass[i]);
-    if (counts && s_count[i]) atomicAdd(&sp.count[i], s_count[i]);
+    if (rule.counts && s_count[i]) atomicAdd(&sp.count[i], s_count[i]);
   }
   if (tid == 0 && s_least) atomicAdd((unsigned long long *)&sp.least_mass, (unsigned long long)s_least);
 }
@@ -266,7 +278,8 @@ struct Choice {                          // LDS of the last launch
   uint64_t part_mass[16];
   uint32_t part_count[16];
   double table[kPerOctave];
-  uint64_t lo, hi, found, upto;
+  uint64_t lo, hi, found, upto, least;
+  float best[16];
   int bin[5], n_pieces, n;
 };
 
@@ -454,7 +467,8 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
   __syncthreads();
 }
 
-template <int dtype>
+// ALL: of a short row the maximum and the histogram as well.
+template <int dtype, bool ALL>
 __global__ void __launch_bounds__(1024)
 sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, int slices, Settings settings,
                      const float *__restrict__ uniform, const RowSpace *__restrict__ space, int64_t *__restrict__ token,
@@ -462,23 +476,60 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
   extern __shared__ char lds[];
   Choice &s = *reinterpret_cast<Choice *>(lds);
   const int tid = threadIdx.x, r = blockIdx.x;
-  const RowSpace &sp = space[r];
   const int64_t was_a = adv.counter_a ? adv.counter_a[0] : 0, was_b = adv.counter_b ? adv.counter_b[0] : 0;
-  // everything that the row's launches left, asked for at once: bins 2 tid and 2 tid + 1
-  const bool has_bins = 2 * tid < kBins;
-  const int at_bins = has_bins ? tid : 0;
-  static_assert(kBins % 2 == 0 && kBins <= 2048, "two bins a thread");
-  const u32x4 masses = reinterpret_cast<const u32x4 *>(sp.mass)[at_bins];
-  const uint64_t two_counts = reinterpret_cast<const uint64_t *>(sp.count)[at_bins];
-  const uint64_t least_sum = sp.least_mass;
-  const float best = row_best(sp, slices);
   const RowSettings set = row_settings(settings, r);
   int64_t at = r;
   if (adv.uniform_index) at = min(max(adv.uniform_index[0], (int64_t)0), (int64_t)adv.n_uniform - 1);
   const float u = uniform[at];
+  const Row<dtype> row(logits, stride, r, vocab);
+  // bins 2 tid and 2 tid + 1
+  const bool has_bins = 2 * tid < kBins;
+  static_assert(kBins % 2 == 0 && kBins <= 2048, "two bins a thread");
+  u32x4 masses;
+  uint64_t two_counts, least_sum;
+  float best;
+  if constexpr (ALL) {
+    float mine = -INFINITY;
+    row.template each<1024>(0, row.pieces, true, [&](float l, int, bool there) __attribute__((always_inline)) {
+      mine = fmaxf(mine, there ? l : -INFINITY);
+    });
+    mine = rdkv_wave_max(mine);
+    if ((tid & 63) == 0) s.best[tid >> 6] = mine;
+    for (int i = tid; i < kBins; i += 1024) {
+      s.mass[i] = 0;
+      s.count[i] = 0;
+    }
+    if (tid == 0) s.least = 0;
+    fill_table(s.table);
+    __syncthreads();
+    best = rdkv_wave_max(s.best[tid & 15]);
+    if (best > -INFINITY && set.T > 0.0f) {
+      const BinRule rule(set);
+      const Scale sc = scale_of(best, set.T, top);
+      uint64_t least_mass = 0;
+      row.template each<1024>(0, row.pieces, true, [&](float l, int, bool there) __attribute__((always_inline)) {
+        rule.add(sc, s.table, s.mass, s.count, least_mass, l, there);
+      });
+      if (rule.least) {
+        least_mass = wave_total(least_mass);
+        if ((tid & 63) == 63 && least_mass) atomicAdd((unsigned long long *)&s.least, (unsigned long long)least_mass);
+      }
+    }
+    __syncthreads();
+    const int of = has_bins ? 2 * tid : 0;
+    masses = u32x4{(uint32_t)s.mass[of], (uint32_t)(s.mass[of] >> 32), (uint32_t)s.mass[of + 1], (uint32_t)(s.mass[of + 1] >> 32)};
+    two_counts = s.count[of] | (uint64_t)s.count[of + 1] << 32;
+    least_sum = s.least;
+  } else {                               // everything that the row's launches left, asked for at once
+    const RowSpace &sp = space[r];
+    masses = reinterpret_cast<const u32x4 *>(sp.mass)[has_bins ? tid : 0];
+    two_counts = reinterpret_cast<const uint64_t *>(sp.count)[has_bins ? tid : 0];
+    least_sum = sp.least_mass;
+    best = row_best(sp, slices);
+    fill_table(s.table);
+  }
   int64_t chosen = -1;
   float lp = -INFINITY;
-  const Row<dtype> row(logits, stride, r, vocab);
   if (best > -INFINITY && !(set.T > 0.0f)) {             // the first place of the largest
     if (tid == 0) s.n = 0x7fffffff;
     __syncthreads();
@@ -492,7 +543,6 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
     lp = 0.0f;
   } else if (best > -INFINITY) {
     const Scale sc = scale_of(best, set.T, top);
-    fill_table(s.table);
     const bool counts = set.top_k > 0;
     if (tid == 0) {
       s.n_pieces = 0;
@@ -1214,15 +1264,19 @@ int slices_of(int rows, int vocab, int elements) {
   return s < 1 ? 1 : s;
 }
 
+// Short rows: all three steps in one launch of a workgroup a row.  One / the others, us, 1 row and 240 rows: fp16, 1000 logits 13.7 /
+// 19.1 and 16.4 / 20.5, 16000 18.6 / 20.2 and 23.3 / 25.4, 32000 23.1 / 20.5 and 29.3 / 27.8; fp32, 1000 logits 11.4 / 16.1 and
+// 14.4 / 19.7, 16000 16.6 / 18.0 and 21.9 / 31.7, 32000 21.2 / 18.8 and 29.2 / 38.5.
+bool in_one(int vocab) { return vocab <= 16384; }
 // A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, fp16, without masks and
 // with 99 % masked: 128256 logits, 1 row 26.8 / 34.0 and 22.0 / 31.2, 8 rows 29.7 / 36.0 and 24.5 / 33.3, 16 rows 38.0 / 36.1 and
-// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 4000 logits, 1 row 18.8 / 20.3 and 18.9 / 16.6.
-bool by_slices(int rows, int dtype) { return dtype == RDKV_DTYPE_F32 || rows <= 12; }
+// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 32000 logits, 8 rows 22.4 / 26.1 and 20.8 / 21.8.
+bool by_slices(int rows, int vocab, int dtype) { return !in_one(vocab) && (dtype == RDKV_DTYPE_F32 || rows <= 12); }
 
 template <int dtype>
 int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set, const float *uniform,
                   int64_t *token, float *logprob, const Advance &adv, RowSpace *space, hipStream_t s) {
-  const bool slices_first = by_slices(rows, dtype);
+  const bool one = in_one(vocab), slices_first = by_slices(rows, vocab, dtype);
   const int slices = slices_of(rows, vocab, Row<dtype>::EPP), top = weight_bits(vocab);
   for (int r = 0; r < rows; r += 65535) {                  // (a grid's second dimension)
     const int n = rows - r < 65535 ? rows - r : 65535;
@@ -1233,12 +1287,15 @@ int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, 
     if (part.top_p) part.top_p += r;
     if (part.min_p) part.min_p += r;
     float *lp = logprob ? logprob + r : nullptr;
-    if (slices_first) {
+    if (one) {
+      hipLaunchKernelGGL((sample_choose_kernel<dtype, true>), dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, 0, part,
+                         uniform + r, nullptr, token + r, lp, adv);
+    } else if (slices_first) {
       hipLaunchKernelGGL(sample_max_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, space + r);
       RDKV_CHECK_LAUNCH(fn);
       hipLaunchKernelGGL(sample_bins_kernel<dtype>, dim3(slices, n), dim3(256), 0, s, from, stride, vocab, top, part, space + r);
       RDKV_CHECK_LAUNCH(fn);
-      hipLaunchKernelGGL(sample_choose_kernel<dtype>, dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
+      hipLaunchKernelGGL((sample_choose_kernel<dtype, false>), dim3(n), dim3(1024), sizeof(Choice), s, from, stride, vocab, top, slices, part,
                          uniform + r, space + r, token + r, lp, adv);
     } else if constexpr (dtype != RDKV_DTYPE_F32) {
       hipLaunchKernelGGL(sample_values_kernel<dtype>, dim3(n), dim3(1024), sizeof(Values), s, from, stride, vocab, top, part, uniform + r,
@@ -1258,7 +1315,7 @@ int sample(const char *fn, const void *logits, int64_t stride, int rows, int voc
   if (rows == 0) return RDKV_OK;
   RDKV_REQUIRE(logits && uniform && token, "%s: null pointer", fn);
   RDKV_REQUIRE(stride >= 0 && ((uintptr_t)logits % (dtype == RDKV_DTYPE_F32 ? 4 : 2)) == 0, "%s: bad rows", fn);
-  const int64_t need = rdkv_sample_workspace_bytes(rows, dtype);
+  const int64_t need = rdkv_sample_workspace_bytes(rows, vocab, dtype);
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0)) {
     rdkv_set_error("%s: needs a 16-byte aligned workspace of %lld bytes", fn, (long long)need);
     return RDKV_EWORKSPACE;
@@ -1273,8 +1330,8 @@ int sample(const char *fn, const void *logits, int64_t stride, int rows, int voc
 
 }  // namespace
 
-RDKV_API int64_t rdkv_sample_workspace_bytes(int rows, int dtype) {
-  return rows <= 0 || !by_slices(rows, dtype) ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace);
+RDKV_API int64_t rdkv_sample_workspace_bytes(int rows, int vocab, int dtype) {
+  return rows <= 0 || !by_slices(rows, vocab, dtype) ? 0 : (int64_t)rows * (int64_t)sizeof(RowSpace);
 }
 
 RDKV_API int rdkv_sample_rows(const void *logits, int64_t stride_row, int rows, int vocab, int dtype,

@@ -97,7 +97,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
             return token, logprob
         uniform = uniform.contiguous()
         lib = _lib.load()
-        need = lib.rdkv_sample_workspace_bytes(B, _lib.DTYPE_CODE[rows.dtype])
+        need = lib.rdkv_sample_workspace_bytes(B, vocab, _lib.DTYPE_CODE[rows.dtype])
         # (the call's own, so that graphs that hold such calls may replay side by side)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.rdkv_sample_rows(rows.data_ptr(), rows.stride(0), B, vocab, _lib.DTYPE_CODE[rows.dtype],
@@ -121,7 +121,7 @@ def _sample_advance(logits: torch.Tensor, token: torch.Tensor, sampling: Samplin
     lib = _lib.load()
     with torch.cuda.device(dev):
         s, _ = _settings(dev, 1, sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)
-        need = lib.rdkv_sample_workspace_bytes(1, _lib.DTYPE_CODE[row.dtype])
+        need = lib.rdkv_sample_workspace_bytes(1, row.numel(), _lib.DTYPE_CODE[row.dtype])
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.rdkv_sample_advance(
             row.data_ptr(), row.numel(), _lib.DTYPE_CODE[row.dtype], uniforms.data_ptr(), uniforms.numel(),

@@ -84,7 +84,7 @@ def _mixed(B, V, seed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 63, 255, 1000, 2049, 4097, 8191, 32000, 128256])
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 63, 255, 1000, 2049, 4097, 8191, 16384, 16385, 32000, 128256])
 def test_mixed_settings(V, dtype):
     require_gpu()
     B = 40 if V < 100_000 else 12
@@ -104,7 +104,7 @@ def test_shared_settings(setting, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("V,spread", [(5000, 0.0), (200_003, 0.0), (60_000, 1e-6), (60_000, 0.003), (3000, 0.0), (65, 0.0)])
+@pytest.mark.parametrize("V,spread", [(5000, 0.0), (200_003, 0.0), (60_000, 1e-6), (60_000, 0.003), (3000, 0.0), (16_000, 1e-6), (65, 0.0)])
 def test_flat_rows(V, spread):
     """Many tokens in one bin (all of them equal, or next to it): the further bins over (logit, index)."""
     require_gpu()
@@ -141,9 +141,9 @@ def test_values_that_occur_very_often(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-def test_masks_infinities_and_no_numbers(dtype):
+@pytest.mark.parametrize("V", [3001, 20_001])
+def test_masks_infinities_and_no_numbers(V, dtype):
     require_gpu()
-    V = 3001
     x, _ = _logits(14, V, dtype, 8)
     low, inf, nan = torch.finfo(dtype).min, float("inf"), float("nan")
     x[0] = -inf                                   # nothing left
@@ -171,7 +171,7 @@ def test_masks_infinities_and_no_numbers(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("V", [131, 9000, 70_001, 140_000])
+@pytest.mark.parametrize("V", [131, 9000, 20_001, 70_001, 140_000])
 def test_rows_that_one_value_fills(V, dtype):
     """One value at most places, as a mask leaves it or as the largest of all: it has to count where it has weight (the
     temperature is high, it is the largest, nothing else is left) and in top-k, and may not where it has none."""
@@ -287,9 +287,10 @@ def test_draws_follow_the_distribution():
 
 
 @pytest.mark.gpu
-def test_streams_and_graphs():
+@pytest.mark.parametrize("B,V", [(33, 30_000), (5, 30_000), (20, 9000)])
+def test_streams_and_graphs(B, V):
     require_gpu()
-    x, u = _logits(33, 30_000, F16, 4)
+    x, u = _logits(B, V, F16, 4)
     xd, ud = x.to(DEV), torch.as_tensor(u, dtype=F32).to(DEV)
     kw = dict(temperature=0.9, top_p=0.95, top_k=200, min_p=0.001)
     exp = sampling.sample_tokens(xd, ud, **kw)[0]
@@ -320,9 +321,10 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
-def test_advance_matches_sample_tokens_and_moves_the_counters():
+@pytest.mark.parametrize("V", [5003, 20_003])
+def test_advance_matches_sample_tokens_and_moves_the_counters(V):
     require_gpu()
-    x, u = _logits(4, 5003, F16, 6)
+    x, u = _logits(4, V, F16, 6)
     s = sampling.Sampling(temperature=0.8, top_k=100, top_p=0.9, min_p=0.01)
     uniforms = torch.as_tensor(u, dtype=F32).to(DEV)
     token, pos, row = (torch.zeros(1, dtype=torch.int64, device=DEV) for _ in range(3))
@@ -358,11 +360,12 @@ def test_refusals_of_the_c_interface():
     lib = _lib.load()
     one = 1 << 20                    # a pointer that is looked at, never followed
     s = _lib.RdkvSampling(temperature_value=1.0, top_p_value=1.0)
-    need = lib.rdkv_sample_workspace_bytes(2, 0)
-    assert need > 0 and lib.rdkv_sample_workspace_bytes(0, 0) == lib.rdkv_sample_workspace_bytes(-3, 0) == lib.rdkv_sample_workspace_bytes(13, 1) == 0
-    assert lib.rdkv_sample_workspace_bytes(2, 1) == lib.rdkv_sample_workspace_bytes(2, 2) == need
+    of = lib.rdkv_sample_workspace_bytes
+    need = of(2, 20000, 0)
+    assert need == of(2, 20000, 1) == of(2, 16385, 2) > 0 and of(40, 20000, 0) == 20 * need
+    assert of(0, 20000, 0) == of(-3, 20000, 0) == of(13, 20000, 1) == of(2, 16384, 0) == of(2, 1, 2) == 0
 
-    def rows(logits=one, stride=64, n=2, vocab=64, dt=0, u=one, settings=ctypes.addressof(s), token=one, ws=one, nb=need):
+    def rows(logits=one, stride=20000, n=2, vocab=20000, dt=0, u=one, settings=ctypes.addressof(s), token=one, ws=one, nb=need):
         return lib.rdkv_sample_rows(logits, stride, n, vocab, dt, u, settings, token, None, ws, nb, None)
 
     for bad in (dict(n=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(dt=3), dict(settings=None), dict(logits=None), dict(u=None),
@@ -373,7 +376,7 @@ def test_refusals_of_the_c_interface():
     assert rows(n=0) == _lib.RDKV_OK
 
     def advance(n_uniform=4, index=one, counter=one, counts=None, n_counts=0, word=None):
-        return lib.rdkv_sample_advance(one, 64, 0, one, n_uniform, index, ctypes.addressof(s), one, counter, None, counts, n_counts, word,
+        return lib.rdkv_sample_advance(one, 20000, 0, one, n_uniform, index, ctypes.addressof(s), one, counter, None, counts, n_counts, word,
                                        0, None, 0, None)
 
     for bad in (dict(n_uniform=0), dict(index=None), dict(n_counts=1025, counts=one), dict(n_counts=1), dict(counter=None, word=one)):
