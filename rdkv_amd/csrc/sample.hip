@@ -467,7 +467,8 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
   __syncthreads();
 }
 
-// ALL: of a short row the maximum and the histogram as well.
+// ALL: of a short row the maximum and the histogram as well.  The three launches of a row of 128256 fp16 logits take 2.8, 5.8 and
+// 14.2 us (the pass over the row about 5), of 64 fp32 rows 6.6, 14.3 and 21.8.
 template <int dtype, bool ALL>
 __global__ void __launch_bounds__(1024)
 sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, int slices, Settings settings,
@@ -831,7 +832,8 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
 // the values' order; a thread owns four blocks of 16 neighbouring patterns and forms their sums (smaller blocks share the
 // crowded values out over more wavefronts, and cost more sums over the workgroup).  Only the
 // token itself needs the row again: the place of its value's n-th occurrence.  A pattern that occurs 2^16 times or more
-// shows in the counters' sum; the patterns are then counted again with 32 bits, half of them at a time.
+// shows in the counters' sum; the patterns are then counted again with 32 bits, half of them at a time.  240 rows of 151937
+// bf16 logits take 47 us, one of 128256 33: counting 9, the sums over values 9, the rest in steps of 3.
 struct Values {                          // LDS
   uint32_t words[1 << 15];               // counter of key k: word_of(k), its half k / 2^15 (or all of it, of one half)
   uint32_t aside[1024];

@@ -70,8 +70,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
     stays.  The token is the first one whose running sum exceeds ``uniform`` times the sum of what stays, the log
     probability its share of that sum.  A ``temperature`` that is not above 0 takes the largest logit (log probability
     0).  Each setting is a number or a tensor with one value per row, on the logits' device (and not looked
-    at by the host: values out of range act as the nearest one in range, NaN as off).  NaN and -inf logits are masked; a row
-    with nothing left has token -1 and log probability -inf."""
+    at by the host: values out of range act as the nearest one in range, NaN as off).  NaN and -inf logits are masked, +inf
+    counts as the largest number of fp32; a row with nothing left has token -1 and log probability -inf."""
     if logits.is_cuda:              # plain arguments: csrc/native.cpp (the checks and the launch cost 27 us interpreted)
         if _lib.native is None:
             _lib.load()
