@@ -468,7 +468,7 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
 }
 
 // ALL: of a short row the maximum and the histogram as well.  The three launches of a row of 128256 fp16 logits take 2.8, 5.8 and
-// 14.2 us (the pass over the row about 5), of 64 fp32 rows 6.6, 14.3 and 21.8.
+// 13.5 us (the pass over the row about 5), of 64 fp32 rows 6.6, 14.3 and 18.
 template <int dtype, bool ALL>
 __global__ void __launch_bounds__(1024)
 sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, int slices, Settings settings,
@@ -701,56 +701,54 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       }
       __syncthreads();
     } else if (!crowded) {
-      // The list in descending order (bitonic over the next power of two, zeros at the end); then what lies in front of
-      // every token: its bin's, and the bin's tokens in front of it.  Up to 1024 tokens: one a thread, partners within a
-      // wavefront through registers, LDS and barriers only for the further ones.
-      int size = 128;
-      while (size < n) size *= 2;
-      if (size <= 1024) {
-        uint64_t v = tid < n ? s.list[tid] : 0;
-        for (int k = 2; k <= size; k *= 2) {
-          const bool down = (tid & k) == 0;
-          for (int j = k / 2; j >= 64; j /= 2) {
-            __syncthreads();
-            if (tid < size) s.list[tid] = v;
-            __syncthreads();
-            const uint64_t other = tid < size ? s.list[tid ^ j] : 0;
-            v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
-          }
-          auto with = [&](int j, uint64_t other) __attribute__((always_inline)) {
-            v = ((tid & j) == 0) == down ? larger(v, other) : lesser(v, other);
+      // The list in descending order: every wavefront sorts 64 tokens in registers (bitonic), then neighbouring runs are merged, a
+      // token's new place being its own and the number of the neighbour's in front of it, between two buffers.  Then what lies in
+      // front of every token: its bin's, and the bin's tokens in front of it.  (1199 tokens: 8.1 us, 9.5 with
+      // four runs at a time, 17.5 with a bitonic sort of all; 594: 4.5, 4.6, 6.6.)
+      for (int i0 = 0; i0 < n; i0 += 1024) {
+        const int i = i0 + tid;
+        if (i - (tid & 63) < n) {
+          uint64_t v = i < n ? s.list[i] : 0;            // (no token is 0: they end up behind the others)
+          auto with = [&](int k, int j, uint64_t other) __attribute__((always_inline)) {
+            v = ((tid & j) == 0) == ((tid & 63 & k) == 0) ? larger(v, other) : lesser(v, other);
           };
-          if (tid < size) {              // (whole wavefronts)
-            if (k >= 64) with(32, __shfl_xor(v, 32, 64));
-            if (k >= 32) with(16, __shfl_xor(v, 16, 64));
-            if (k >= 16) with(8, partner<uint64_t, 0x128>(v));
-            if (k >= 8) with(4, partner<uint64_t, 0x1b>(partner<uint64_t, 0x141>(v)));      // 7 ^ 3
-            if (k >= 4) with(2, partner<uint64_t, 0x4e>(v));
-            with(1, partner<uint64_t, 0xb1>(v));
+#pragma unroll
+          for (int k = 2; k <= 64; k *= 2) {
+            if (k >= 64) with(k, 32, __shfl_xor(v, 32, 64));
+            if (k >= 32) with(k, 16, __shfl_xor(v, 16, 64));
+            if (k >= 16) with(k, 8, partner<uint64_t, 0x128>(v));
+            if (k >= 8) with(k, 4, partner<uint64_t, 0x1b>(partner<uint64_t, 0x141>(v)));      // 7 ^ 3
+            if (k >= 4) with(k, 2, partner<uint64_t, 0x4e>(v));
+            with(k, 1, partner<uint64_t, 0xb1>(v));
           }
-        }
-        __syncthreads();
-        if (tid < n) s.list[tid] = v;
-        __syncthreads();
-      } else {
-        for (int i = n + tid; i < size; i += 1024) s.list[i] = 0;
-        __syncthreads();
-        for (int k = 2; k <= size; k *= 2) {
-          for (int j = k / 2; j > 0; j /= 2) {
-            for (int q = tid; q < size / 2; q += 1024) {
-              const int x = 2 * q - (q & (j - 1)), y = x + j;
-              const uint64_t lx = s.list[x], ly = s.list[y];
-              if ((lx < ly) == ((x & k) == 0)) {
-                s.list[x] = ly;
-                s.list[y] = lx;
-              }
-            }
-            __syncthreads();
-          }
+          if (i < n) s.list[i] = v;
         }
       }
+      uint64_t *sorted = s.list, *other = s.before;
+      for (int run = 64; run < n; run *= 2) {
+        __syncthreads();
+        for (int i = tid; i < n; i += 1024) {
+          const uint64_t v = sorted[i];
+          const int mine = i & -run, next = min(mine ^ run, n), end = min(next + run, n);
+          int lo = next, hi = end;                       // the first of the neighbour's that is not in front
+          while (lo < hi) {
+            const int middle = (lo + hi) / 2;
+            if (sorted[middle] > v) lo = middle + 1;
+            else hi = middle;
+          }
+          other[(mine & ~run) + (i - mine) + (lo - next)] = v;
+        }
+        uint64_t *const was = sorted;
+        sorted = other;
+        other = was;
+      }
+      __syncthreads();
+      if (sorted != s.list) {
+        for (int i = tid; i < n; i += 1024) s.list[i] = sorted[i];
+        __syncthreads();
+      }
       auto bin_at = [&](int i) __attribute__((always_inline)) { return (int)placed(bins_below(sc, composite_logit(s.list[i]))); };
-      const int each = size > 1024 ? size / 1024 : 1, first = tid * each, last = min(first + each, n);
+      const int each = (n + 1023) / 1024, first = tid * each, last = min(first + each, n);
       uint64_t sum = 0;
 #pragma unroll 1
       for (int i = first; i < last; ++i) {
