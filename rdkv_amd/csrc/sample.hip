@@ -467,8 +467,10 @@ __device__ __forceinline__ void crowded_search(Choice &s, const Row<dtype> &row,
   __syncthreads();
 }
 
+template <int N> struct Count { static constexpr int value = N; };
+
 // ALL: of a short row the maximum and the histogram as well.  The three launches of a row of 128256 fp16 logits take 2.8, 5.8 and
-// 13.5 us (the pass over the row about 5), of 64 fp32 rows 6.6, 14.3 and 18.
+// 12 us (the pass over the row about 4), of 64 fp32 rows 6.6, 14.3 and 17.
 template <int dtype, bool ALL>
 __global__ void __launch_bounds__(1024)
 sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab, int top, int slices, Settings settings,
@@ -600,11 +602,13 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
     mark(4, token_target(u, run_hi));
     __syncthreads();
     from[2] = s.bin[3], to[2] = s.bin[4];
-    // Pieces of the row that may hold a token of these bins: smallest distances from the three middles.
-    const Near a = near_bins(sc, set.T, by_k ? from[0] : from[2], by_k ? to[0] : to[2]),
-               b = near_bins(sc, set.T, by_p ? from[1] : from[2], by_p ? to[1] : to[2]), c = near_bins(sc, set.T, from[2], to[2]);
+    // Pieces of the row that may hold a token of these bins: smallest distances from the middles, of the searches that there
+    // are (the pass is bound by these: three always took 1.6 us more of the 25 of a row of 128256 under top-p).
+    const Near near[3] = {near_bins(sc, set.T, from[2], to[2]), near_bins(sc, set.T, by_p ? from[1] : from[0], by_p ? to[1] : to[0]),
+                          near_bins(sc, set.T, from[0], to[0])};
     constexpr int EPP = Row<dtype>::EPP, U = 8;
-    auto scan = [&](auto both) __attribute__((always_inline)) {
+    auto scan = [&](auto ranges) __attribute__((always_inline)) {
+      constexpr int R = decltype(ranges)::value;
       for (int i0 = 0; i0 < row.pieces; i0 += U * 1024) {
         u32x4 v[U];
 #pragma unroll
@@ -615,18 +619,18 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
         uint32_t hits = 0;
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          float da = INFINITY, db = INFINITY, dc = INFINITY;
+          float distance[R];
+#pragma unroll
+          for (int q = 0; q < R; ++q) distance[q] = INFINITY;
 #pragma unroll
           for (int e = 0; e < EPP; ++e) {
             const float l = row.value(v[k], e);
-            if (both) {
-              da = fminf(da, fabsf(l - a.middle));
-              db = fminf(db, fabsf(l - b.middle));
-            }
-            dc = fminf(dc, fabsf(l - c.middle));
+#pragma unroll
+            for (int q = 0; q < R; ++q) distance[q] = fminf(distance[q], fabsf(l - near[q].middle));
           }
-          bool hit = dc <= c.half;
-          if (both) hit |= (da <= a.half) | (db <= b.half);
+          bool hit = false;
+#pragma unroll
+          for (int q = 0; q < R; ++q) hit |= distance[q] <= near[q].half;
           hits |= hit && i0 + k * 1024 + tid < row.pieces ? 1u << k : 0u;
         }
         if (__any(hits != 0)) {          // places in the list for all of the wavefront's pieces at once
@@ -645,10 +649,9 @@ sample_choose_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
         }
       }
     };
-    struct Yes { __device__ constexpr operator bool() const { return true; } };
-    struct No { __device__ constexpr operator bool() const { return false; } };
-    if (by_k || by_p) scan(Yes{});
-    else scan(No{});
+    if (by_k && by_p) scan(Count<3>{});
+    else if (by_k || by_p) scan(Count<2>{});
+    else scan(Count<1>{});
     __syncthreads();
     // Their tokens in these bins (and those in front of and behind the pieces).
     const int n_pieces = s.n_pieces;
