@@ -874,8 +874,8 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
 #pragma unroll
     for (int i = 0; i < (1 << 13) / 1024; ++i) words[i * 1024 + tid] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    // Masked tokens share one value: a value that a quarter of a wavefront's lanes start with is counted aside, in a word of
-    // the lane's own, and left out if it is no number or fills half of the row (rows of 128256 with 99 % masked: 31 us; 250 with
+    // Masked tokens share one value: a value that an eighth of a wavefront's lanes start with is counted aside, in a word of
+    // the lane's own, and left out if it is no number or fills half of the row (rows of 128256 with 99 % masked: 34 us; 250 with
     // their counts added up at one address, beyond the 16 bits of a counter).  Any key will do.
     uint32_t aside = 0;
     bool some = false;
@@ -905,13 +905,11 @@ sample_values_kernel(const void *__restrict__ logits, int64_t stride, int vocab,
       }
       if (i0 == 0) {
         const uint32_t pair = v[0][0], first = keys_of(pair) & 0xffffu;
-#pragma unroll
-        for (int of = 0; of < 64; of += 16) {
-          const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)first, of);
-          if (__popcll(__ballot(first == key)) >= 16) {
-            aside = key;
-            some = true;
-          }
+        const uint64_t twins = __ballot((first == moved<0xb1, 0xf>(first)) | (first == moved<0x4e, 0xf>(first)) | (first == moved<0x1b, 0xf>(first)));
+        if (twins) {                       // lanes of four that start with the same value
+          const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)first, __ffsll((unsigned long long)twins) - 1);
+          some = __popcll(__ballot(first == key)) >= 8;
+          aside = some ? key : 0;
         }
       }
       auto all = [&](bool look_aside) __attribute__((always_inline)) {
@@ -1271,10 +1269,10 @@ int slices_of(int rows, int vocab, int elements) {
 // 19.1 and 16.4 / 20.5, 16000 18.6 / 20.2 and 23.3 / 25.4, 32000 23.1 / 20.5 and 29.3 / 27.8; fp32, 1000 logits 11.4 / 16.1 and
 // 14.4 / 19.7, 16000 16.6 / 18.0 and 21.9 / 31.7, 32000 21.2 / 18.8 and 29.2 / 38.5.
 bool in_one(int vocab) { return vocab <= 16384; }
-// A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, fp16, without masks and
-// with 99 % masked: 128256 logits, 1 row 26.8 / 34.0 and 22.0 / 31.2, 8 rows 29.7 / 36.0 and 24.5 / 33.3, 16 rows 38.0 / 36.1 and
-// 26.8 / 33.4, 64 rows 46.3 / 37.5 and 32.3 / 34.2; 32000 logits, 8 rows 22.4 / 26.1 and 20.8 / 21.8.
-bool by_slices(int rows, int vocab, int dtype) { return !in_one(vocab) && (dtype == RDKV_DTYPE_F32 || rows <= 12); }
+// A few rows of 16-bit logits leave most compute units idle with one workgroup a row.  Slices / values, us, without masks and with
+// 99 % masked: 128256 fp16 logits, 8 rows 30 / 37 and 24 / 34, 24 rows 35 / 37 and 27 / 34, 48 rows 41 / 38 and 31 / 35; 32000 bf16
+// logits, 8 rows 22 / 26 and 20 / 24, 48 rows 28 / 27 and 22 / 25.
+bool by_slices(int rows, int vocab, int dtype) { return !in_one(vocab) && (dtype == RDKV_DTYPE_F32 || rows <= 24); }
 
 template <int dtype>
 int launch_sample(const char *fn, const void *logits, int64_t stride, int rows, int vocab, const Settings &set, const float *uniform,
